@@ -250,6 +250,112 @@ int matmul_decoder_step_sample(MatmulDecoderContext* ctx, int token_id, const fl
 int mdx_sample_topk_noalloc(const float* logits, int V, float temperature, int top_k, float top_p,
                             float uniform, int* out, int* top_idx, float* top_val, void* stream);
 
+/* ---- many requests over a paged K/V cache ------------------------------- */
+
+/* No counterpart in the reference, whose cache is one request's contiguous
+ * rows.  Here requests share a pool of pages, and a step takes the new rows of
+ * all of them at once: mdx_paged_append puts their keys and values into the
+ * pages, mdx_paged_attention attends over them, mdx_paged_mass adds up the
+ * attention weight that each cached row receives, and mdx_paged_evict cuts a
+ * cache back to a budget of rows by it.
+ *
+ * All pointers are device pointers on the current device.  Every call enqueues
+ * kernels on `stream` (NULL: the default stream) and returns without
+ * synchronising; none allocates, copies or records a memset node, so all can be
+ * captured into a graph and replayed with other contents of the same arrays.
+ * Workspaces are the caller's (mdx_paged_*_workspace bytes, 16-byte aligned, no
+ * initial value); calls that may overlap need one each.  Return 0, INVALID_ARG
+ * (-1) for bad arguments, UNSUPPORTED (-5) for a head size or page size below
+ * that has no kernel, ERR_RKNN (-4) on a HIP failure; the message is
+ * mdx_last_error().
+ *
+ * What lies in device memory cannot be checked before the launch, so the
+ * kernels check it: a page number outside [0, n_pages) is never followed; its
+ * rows count as absent (not written, not attended over, not moved). */
+typedef enum {
+    MDX_TYPE_F16 = 0,
+    MDX_TYPE_BF16 = 1,
+} MdxType;
+
+typedef struct {
+    MdxType type;           /* of K, V, the query rows and the attention's rows */
+    int num_q_heads;        /* a multiple of num_kv_heads */
+    int num_kv_heads;
+    int head_dim;           /* 64, 128 or 256 */
+    int page_size;          /* rows per page: a power of two, 16 to 1024 */
+    int n_pages;            /* pages in the pool */
+    void* k_pages;          /* [n_pages][num_kv_heads][page_size][head_dim], 16-byte aligned */
+    void* v_pages;
+    float* mass;            /* [n_pages][num_kv_heads][page_size]: weight received (NULL: not kept) */
+    int* pos;               /* the same: the row's position in its request (NULL: not kept) */
+} MdxPagedCache;
+
+/* The new rows of n_req requests, request after request.  Row i of the
+ * n = q_start[r+1] - q_start[r] new rows of request r is row kv_len[r] - n + i
+ * of its cache (a negative one is in no cache: it sees nothing), and row j of
+ * a cache is row j % page_size of page block_table[r][j / page_size].
+ * Attention only reads pages and takes ones that several requests share; the
+ * pages that the other calls write (new rows, mass, evicted requests) have to
+ * be the request's own. */
+typedef struct {
+    int n_req;
+    int n_tokens;           /* new rows of all requests; rows behind q_start[n_req] are left alone */
+    int max_q_len;          /* no request has more new rows (further ones are left out) */
+    int max_kv_len;         /* nor more cache rows, the new ones included (further ones are absent) */
+    int max_pages;          /* entries per request in block_table */
+    const int* q_start;     /* [n_req + 1], ascending from 0 */
+    const int* kv_len;      /* [n_req] */
+    const int* block_table; /* [n_req][max_pages] */
+} MdxPagedBatch;
+
+/* From the fp32 qkv projection of the new rows ([n_tokens] rows, qkv_stride
+ * floats apart: q heads, K heads, V heads): per head of q and k
+ * x * (1 / sqrt(mean(x^2) + eps)) * norm (a NULL norm: x as it is), then the
+ * rotation by row positions[t] of cos_t / sin_t ([max_pos][head_dim / 2]; pairs
+ * (2i, 2i+1) for rope_style 0, (i, i + head_dim/2) for 1), all in fp32 and
+ * rounded once.  K and V go to the row's place in its request's pages, with
+ * mass 0 and pos positions[t] where those are kept; q to q_out ([n_tokens] rows,
+ * q_stride values apart).  A row whose position is outside the tables is left
+ * out. */
+int mdx_paged_append(const MdxPagedCache* cache, const MdxPagedBatch* batch, const float* qkv,
+                     long long qkv_stride, const int* positions, const float* q_norm,
+                     const float* k_norm, float eps, const float* cos_t, const float* sin_t,
+                     int max_pos, int rope_style, void* q_out, long long q_stride, void* stream);
+
+/* out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j]) V[j] over the cache rows j
+ * that row t sees, those up to itself (scale 0: 1 / sqrt(head_dim)); lse[t][h]
+ * (NULL: not wanted) the natural logarithm of the sum of the exponentials.  A
+ * row that sees nothing gets zeros and lse -inf.  Rows are q_stride / out_stride
+ * values apart, lse rows num_q_heads. */
+size_t mdx_paged_attention_workspace(const MdxPagedCache* cache, const MdxPagedBatch* batch);
+int mdx_paged_attention(const MdxPagedCache* cache, const MdxPagedBatch* batch, const void* q,
+                        long long q_stride, float scale, void* out, long long out_stride, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* mass[j] of each KV head += sum over the query heads of its group and the new
+ * rows t that see cache row j of exp(scale * q[t][h] . K[j] - lse[t][h]), with
+ * the q, scale and lse of mdx_paged_attention. */
+size_t mdx_paged_mass_workspace(const MdxPagedCache* cache, const MdxPagedBatch* batch);
+int mdx_paged_mass(const MdxPagedCache* cache, const MdxPagedBatch* batch, const void* q,
+                   long long q_stride, float scale, const float* lse, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Cuts every request with more than `budget` cache rows back to budget, for
+ * each KV head by itself.  Rows of the first `sink` positions and the `recent`
+ * newest ones (pos < sink, pos > the largest pos - recent) stay before others;
+ * then rows go by mass (a NaN is the least), ties to the lower row.  Rows that
+ * stay among the first budget ones keep their place; the j-th of the others that
+ * stay takes the place of the j-th of the first budget that goes, K, V, mass and
+ * pos.  The caller sets the request's kv_len to budget then; a row's place says
+ * nothing of its position any more, pos does.  Rows [0, min(kv_len, budget)) of
+ * mass_out / pos_out are written: cache->mass and cache->pos themselves, or
+ * arrays of their size that leave these as they were.  sink + recent <= budget.
+ * q_start, n_tokens and max_q_len are not read. */
+size_t mdx_paged_evict_workspace(const MdxPagedCache* cache, const MdxPagedBatch* batch, int budget);
+int mdx_paged_evict(const MdxPagedCache* cache, const MdxPagedBatch* batch, int budget, int sink,
+                    int recent, float* mass_out, int* pos_out, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* Device memory and synchronous copies on the current device, for callers
  * and tests that hand device pointers to the device-pointer entry points.
  * Return 0 or a negative error. */

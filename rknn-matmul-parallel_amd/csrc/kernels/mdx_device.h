@@ -57,6 +57,10 @@ typedef struct {
 /* ---- runtime wrappers (mdx_rt.hip) ---- */
 int mdxrt_device_count(void);
 const char* mdxrt_last_error(void);
+/* Records `message` as the last error and returns rc. */
+int mdxrt_refuse(int rc, const char* message);
+/* 0, or the recorded failure of the launches before it. */
+int mdxrt_launched(const char* what);
 int mdxrt_malloc(void** p, size_t bytes);
 int mdxrt_free(void* p);
 int mdxrt_host_alloc(void** p, size_t bytes);     /* pinned */

@@ -1,0 +1,891 @@
+// mdx_paged.hip — a K/V cache in pages that many requests share: append of the
+// new rows (QK-norm + RoPE), attention over the pages, the weight that cached
+// rows receive, and eviction by it; gfx950.
+//
+// Pages are [n_pages][nkv][page][hd], so that a KV head's rows within a page
+// are contiguous.  Row i of a request's n new rows is cache row L - n + i.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "mdx_common.h"
+#include "mdx_device.h"
+#include "mdx_paged.h"
+
+using namespace mdx;
+
+namespace {
+
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// The cache and the batch as the kernels take them.
+struct Paged {
+    uint16_t* kp;
+    uint16_t* vp;
+    float* mass;
+    int* pos;
+    const int* q_start;
+    const int* kv_len;
+    const int* table;
+    int n_req, n_tokens, max_q, max_pages, n_pages;
+    int nq, nkv, G, shift;     // page size 1 << shift
+    int limit;                 // cache rows that exist: min(max_kv_len, max_pages * page)
+};
+
+Paged paged(const MdxPagedCache* c, const MdxPagedBatch* b) {
+    Paged p = {};
+    p.kp = (uint16_t*)c->k_pages;
+    p.vp = (uint16_t*)c->v_pages;
+    p.mass = c->mass;
+    p.pos = c->pos;
+    p.q_start = b->q_start;
+    p.kv_len = b->kv_len;
+    p.table = b->block_table;
+    p.n_req = b->n_req;
+    p.n_tokens = b->n_tokens;
+    p.max_q = b->max_q_len;
+    p.max_pages = b->max_pages;
+    p.n_pages = c->n_pages;
+    p.nq = c->num_q_heads;
+    p.nkv = c->num_kv_heads;
+    p.G = c->num_q_heads / c->num_kv_heads;
+    p.shift = __builtin_ctz((unsigned)c->page_size);
+    const long long rows = (long long)b->max_pages * c->page_size;
+    p.limit = rows < b->max_kv_len ? (int)rows : b->max_kv_len;
+    return p;
+}
+
+// A request's new rows: [start, start + n) of the batch; base: the cache row of
+// the first (negative if the cache is shorter than they are).
+struct Req {
+    int start, n, base;
+};
+__device__ __forceinline__ Req req_of(const Paged& p, int r) {
+    Req q;
+    q.start = min(max(p.q_start[r], 0), p.n_tokens);
+    q.n = max(min(p.q_start[r + 1], p.n_tokens) - q.start, 0);
+    q.base = max(p.kv_len[r], 0) - q.n;
+    return q;
+}
+
+// The request of batch row t, by a whole wave: how many requests end at or
+// before it (n_req: the row is behind the last one).
+__device__ __forceinline__ int find_req(const Paged& p, int t, int lane) {
+    int r = 0;
+    for (int j = 0; j < p.n_req; j += 64)
+        r += __popcll(__ballot(j + lane < p.n_req && p.q_start[min(j + lane, p.n_req - 1) + 1] <= t));
+    return r;
+}
+
+// Row number (of the pool, for one head) of cache row j, or -1.
+__device__ __forceinline__ long long pool_row(const Paged& p, int r, int h, int j) {
+    const int pg = p.table[(size_t)r * p.max_pages + (j >> p.shift)];
+    if ((unsigned)pg >= (unsigned)p.n_pages) return -1;
+    return ((((long long)pg * p.nkv + h) << p.shift)) + (j & ((1 << p.shift) - 1));
+}
+
+template <class T>
+__device__ __forceinline__ uint16_t bits16(float f) {
+    return __builtin_bit_cast(uint16_t, (T)f);
+}
+template <class T>
+__device__ __forceinline__ float widen16(uint16_t b) {
+    return (float)__builtin_bit_cast(T, b);
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    return (uint32_t)bits16<T>(a) | ((uint32_t)bits16<T>(b) << 16);
+}
+
+__device__ __forceinline__ float4_t mfma16(_Float16, u32x4_t a, u32x4_t b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+}
+__device__ __forceinline__ float4_t mfma16(__bf16, u32x4_t a, u32x4_t b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0,
+                                                   0);
+}
+
+// ---- append -----------------------------------------------------------------------
+//
+// One workgroup per new row; HD/4 lanes per head, four values each, so that a
+// head is read with 16-byte loads, its sum of squares is a few cross-lane adds
+// and a rotation's partner is in this lane (pairs) or HD/8 lanes away (halves).
+// Reads and writes are all it does: 4 + 2 bytes per value.
+struct AppendArgs {
+    Paged p;
+    const float* qkv;
+    long long qkv_stride;
+    const int* positions;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+    const float* cos_t;
+    const float* sin_t;
+    int max_pos, style;
+    uint16_t* q_out;
+    long long q_stride;
+};
+
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
+    constexpr int LPH = HD / 4;            // lanes per head
+    const Paged& p = a.p;
+    const int t = blockIdx.x, lane = threadIdx.x & 63;
+    const int r = find_req(p, t, lane);
+    if (r >= p.n_req) return;
+    const Req q = req_of(p, r);
+    const int i = t - q.start;
+    const int pos = a.positions[t];
+    if (i < 0 || i >= min(q.n, p.max_q) || pos < 0 || pos >= a.max_pos) return;
+    const int j = q.base + i;              // cache row
+    const bool held = j >= 0 && j < p.limit;
+    const int l = threadIdx.x % LPH, heads = p.nq + 2 * p.nkv;
+    const float* row = a.qkv + (size_t)t * a.qkv_stride;
+    const float* cr = a.cos_t + (size_t)pos * (HD / 2);
+    const float* sr = a.sin_t + (size_t)pos * (HD / 2);
+    for (int h0 = 0; h0 < heads; h0 += 256 / LPH) {
+        const int h = h0 + threadIdx.x / LPH;
+        const bool hv = h < heads;
+        float4 x = *reinterpret_cast<const float4*>(row + (size_t)min(h, heads - 1) * HD + 4 * l);
+        const float* nw = h < p.nq ? a.q_norm : a.k_norm;
+        const bool turn = h < p.nq + p.nkv;
+        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
+        ss = group_sum(ss, LPH);
+        if (turn && nw) {
+            const float rms = 1.0f / sqrtf(ss / (float)HD + a.eps);
+            const float4 w = *reinterpret_cast<const float4*>(nw + 4 * l);
+            x.x = (x.x * rms) * w.x;
+            x.y = (x.y * rms) * w.y;
+            x.z = (x.z * rms) * w.z;
+            x.w = (x.w * rms) * w.w;
+        }
+        if (a.style == 0) {
+            if (turn) {
+                const float2 c = *reinterpret_cast<const float2*>(cr + 2 * l);
+                const float2 s = *reinterpret_cast<const float2*>(sr + 2 * l);
+                x = make_float4(x.x * c.x - x.y * s.x, x.y * c.x + x.x * s.x, x.z * c.y - x.w * s.y,
+                                x.w * c.y + x.z * s.y);
+            }
+        } else {
+            float4 y;
+            y.x = __shfl_xor(x.x, LPH / 2, kWave);
+            y.y = __shfl_xor(x.y, LPH / 2, kWave);
+            y.z = __shfl_xor(x.z, LPH / 2, kWave);
+            y.w = __shfl_xor(x.w, LPH / 2, kWave);
+            if (turn) {
+                const int lo = l % (LPH / 2);
+                const float4 c = *reinterpret_cast<const float4*>(cr + 4 * lo);
+                float4 s = *reinterpret_cast<const float4*>(sr + 4 * lo);
+                if (l < LPH / 2) s = make_float4(-s.x, -s.y, -s.z, -s.w);
+                x = make_float4(x.x * c.x + y.x * s.x, x.y * c.y + y.y * s.y, x.z * c.z + y.z * s.z,
+                                x.w * c.w + y.w * s.w);
+            }
+        }
+        if (!hv) continue;
+        const uint2 o = make_uint2(pack16<T>(x.x, x.y), pack16<T>(x.z, x.w));
+        if (h < p.nq) {
+            *reinterpret_cast<uint2*>(a.q_out + (size_t)t * a.q_stride + (size_t)h * HD + 4 * l) = o;
+        } else if (held) {
+            const bool is_k = h < p.nq + p.nkv;
+            const long long to = pool_row(p, r, is_k ? h - p.nq : h - p.nq - p.nkv, j);
+            if (to < 0) continue;
+            *reinterpret_cast<uint2*>((is_k ? p.kp : p.vp) + to * HD + 4 * l) = o;
+            if (is_k && l == 0) {
+                if (p.mass) p.mass[to] = 0.0f;
+                if (p.pos) p.pos[to] = pos;
+            }
+        }
+    }
+}
+
+// ---- attention ----------------------------------------------------------------------
+//
+// A workgroup takes 16 query rows (new rows x the heads of one KV head's group)
+// and a split of the keys; its waves take alternate tiles of 32 keys, each with
+// a running maximum and sum of its own, and are joined through LDS; splits are
+// joined by a second kernel.  K and V go from the pages into registers as the
+// matrix operands, without LDS:
+//   S^T = K . Q^T      lane (g, c): key row c of 16, dims 32s + 8g ..
+//   O^T = V^T . P^T    lane (g, c): 8 keys x the dims (HD/16) c .., transposed
+//                      in registers by v_perm; the k order is that in which S^T
+//                      leaves a lane's keys (4g + i, 16 + 4g + i), and product
+//                      j has the dims (HD/16) m + j, so a lane's outputs of all
+//                      products are contiguous.
+// Probabilities enter as the sum of two 16-bit values (22 bits in fp16, 16 in
+// bf16): the keys' bytes bound this kernel, not its products.
+//
+// Rows and their order: masks are -inf scores; V rows that no row of the tile
+// sees are zeroed as they are loaded.  What is left of a non-finite V value at a
+// masked place would be 0 * inf; outputs that are not finite therefore make the
+// wave run again with every tile checked, and tiles that hold such values take
+// the products of visible keys alone, in fp32.
+struct AttnArgs {
+    Paged p;
+    const uint16_t* q;
+    long long q_stride;
+    float scale, c;            // c: scale * log2 e
+    uint16_t* out;
+    long long out_stride;
+    float* lse;
+    float* part_o;             // [splits][n_tokens * nq][hd]
+    float2* part_ml;           // [splits][n_tokens * nq]: reference score, sum
+    int splits, split_keys;
+};
+
+// Probabilities are 2^(c (s - ref) + lift); the difference comes first, so that
+// it is exact near the maximum however large the scores are.  The reference only
+// moves when a row's maximum has outgrown it by 2^8; the lift takes fp16 values
+// away from the subnormal ones.
+template <class T> constexpr float kLift = 0.0f;
+template <> constexpr float kLift<_Float16> = 7.0f;
+
+// The result of a row from its unnormalised sum.  top: the reference; l: the sum,
+// or for a reference of -inf a mark: 0 when no key was seen, else more (all at
+// -inf) or NaN.
+__device__ __forceinline__ float row_result(float o, float top, float l) {
+    return top == -INFINITY ? (l == 0.0f ? 0.0f : NAN) : o / l;
+}
+template <class T>
+__device__ __forceinline__ float row_lse(float top, float l, float scale) {
+    return top == -INFINITY ? (l != l ? l : -INFINITY) : __builtin_fmaf(top, scale, (__log2f(l) - kLift<T>) * kLn2);
+}
+// What sums relative to `ref` weigh in ones relative to `top` >= ref.
+__device__ __forceinline__ float ref_weight(float ref, float top, float c) {
+    return ref == top ? 1.0f : __builtin_amdgcn_exp2f((ref - top) * c);
+}
+
+template <int HD, class T>
+__global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
+    constexpr int DS = HD / 32, DJ = HD / 16;
+    constexpr int OS = HD + 4;                       // floats per row of the joined sums
+    __shared__ float osh[4 * 16 * OS];
+    __shared__ float msh[4][16], lsh[4][16];
+    const Paged& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int g = lane >> 4, c16 = lane & 15;
+    const int r = blockIdx.z, kvh = blockIdx.y % p.nkv, tile = blockIdx.y / p.nkv, split = blockIdx.x;
+    const Req q = req_of(p, r);
+    const int rows = min(q.n, p.max_q) * p.G;
+    if (tile * 16 >= rows) return;
+    const int R = min(tile * 16 + c16, rows - 1);    // this lane's query row (the last one repeated)
+    const int tok = q.start + R / p.G, hq = kvh * p.G + R % p.G;
+    const int vis = min(q.base + R / p.G + 1, p.limit);
+    const int vmin = min(q.base + tile * 16 / p.G + 1, p.limit);
+    const int kend = min(q.base + min(tile * 16 + 15, rows - 1) / p.G + 1, p.limit);
+    const int k0 = split * a.split_keys, k1 = min(kend, k0 + a.split_keys);
+    if (k0 >= k1 && split > 0) return;
+
+    u32x4_t qf[DS];
+    {
+        const uint16_t* qr = a.q + (size_t)tok * a.q_stride + (size_t)hq * HD + 8 * g;
+#pragma unroll
+        for (int s = 0; s < DS; s++) qf[s] = *reinterpret_cast<const u32x4_t*>(qr + 32 * s);
+    }
+    const int* table = p.table + (size_t)r * p.max_pages;
+    const int pmask = (1 << p.shift) - 1;
+
+    float4_t o[DJ];
+    float ref, l;
+    bool seen;
+    for (int careful = 0;; careful = 1) {
+#pragma unroll
+        for (int j = 0; j < DJ; j++) o[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        ref = -INFINITY;
+        l = 0.0f;
+        seen = false;
+        for (int kb = k0 + 32 * wave; kb < k1; kb += 128) {
+            u32x4_t kf[2][DS];
+            uint32_t vr[8][DJ / 2];
+            size_t vrow[2];
+            bool ok[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int kk = kb + 16 * u;
+                const int pg = kk < k1 ? table[kk >> p.shift] : -1;
+                ok[u] = (unsigned)pg < (unsigned)p.n_pages;
+                const size_t row = (((size_t)(ok[u] ? pg : 0) * p.nkv + kvh) << p.shift) + (kk & pmask);
+                vrow[u] = row * HD;
+                const uint16_t* kp = p.kp + (row + c16) * HD + 8 * g;
+#pragma unroll
+                for (int s = 0; s < DS; s++) kf[u][s] = *reinterpret_cast<const u32x4_t*>(kp + 32 * s);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint16_t* vp = p.vp + (row + 4 * g + e) * HD + DJ * c16;
+                    if constexpr (DJ == 4) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(vp);
+                        vr[4 * u + e][0] = v.x;
+                        vr[4 * u + e][1] = v.y;
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < DJ / 8; d++) {
+                            const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vp + 8 * d);
+#pragma unroll
+                            for (int w = 0; w < 4; w++) vr[4 * u + e][4 * d + w] = v[w];
+                        }
+                    }
+                }
+            }
+            const bool edge = kb + 32 > vmin || !ok[0] || !ok[1];
+            if (kb + 32 > kend || !ok[0] || !ok[1]) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!ok[e >> 2] || kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend)
+#pragma unroll
+                        for (int d = 0; d < DJ / 2; d++) vr[e][d] = 0;
+            }
+            float4_t s[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int d = 0; d < DS; d++) s[u] = mfma16(T(), kf[u][d], qf[d], s[u]);
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (!ok[u] || kb + 16 * u + 4 * g + i >= vis) s[u][i] = -INFINITY;
+                }
+                seen |= ok[u] && kb + 16 * u < vis;
+            }
+            float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                             fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            mx = rows_max4(mx);
+            const float next = (mx - ref) * a.c > 8.0f ? mx : ref;
+            const float off = next == -INFINITY ? 0.0f : next;
+            if (__any(next != ref)) {
+                const float alpha = ref_weight(ref, next, a.c);
+                l = l * alpha;
+#pragma unroll
+                for (int j = 0; j < DJ; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[j][i] = o[j][i] * alpha;
+                ref = next;
+            }
+            u32x4_t ph, pl;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i] - off, a.c, kLift<T>));
+                    l = l + s[u][i];
+                    lo[i] = s[u][i] - (float)(T)s[u][i];
+                }
+                ph[2 * u] = pack16<T>(s[u][0], s[u][1]);
+                ph[2 * u + 1] = pack16<T>(s[u][2], s[u][3]);
+                pl[2 * u] = pack16<T>(lo[0], lo[1]);
+                pl[2 * u + 1] = pack16<T>(lo[2], lo[3]);
+            }
+            bool slow = false;
+            if (careful) {
+                constexpr uint32_t ex = sizeof(T) == 2 && kLift<T> != 0.0f ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+#pragma unroll
+                    for (int d = 0; d < DJ / 2; d++)
+                        slow |= (vr[e][d] & ex) == ex || ((vr[e][d] >> 16) & ex) == ex;
+                slow = __any(slow);
+            }
+            if (!slow) {
+#pragma unroll
+                for (int j = 0; j < DJ; j++) {
+                    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+                    u32x4_t vf;
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        vf[w] = __builtin_amdgcn_perm(vr[2 * w + 1][j / 2], vr[2 * w][j / 2], sel);
+                    o[j] = mfma16(T(), vf, pl, o[j]);
+                    o[j] = mfma16(T(), vf, ph, o[j]);
+                }
+            } else {
+                float* ps = osh + wave * 16 * OS;            // [32 keys][16 rows]
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) ps[(16 * u + 4 * g + i) * 16 + c16] = s[u][i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+                for (int key = 0; key < 32; key++) {
+                    if (!ok[key >> 4] || kb + key >= vis) continue;
+                    const float pk = ps[key * 16 + c16];
+                    const uint16_t* vp = p.vp + vrow[key >> 4] + (size_t)(key & 15) * HD;
+#pragma unroll
+                    for (int j = 0; j < DJ; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[j][i] = o[j][i] + pk * widen16<T>(vp[DJ * (4 * g + i) + j]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        if (careful) break;
+        float any = 0.0f;                            // NaN when an output is not finite
+#pragma unroll
+        for (int j = 0; j < DJ; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) any = any + o[j][i] * 0.0f;
+        if (!__any(any != any)) break;
+    }
+
+    l = rows_sum4(l);
+    if (ref == -INFINITY && l == l) l = seen ? 1.0f : 0.0f;
+    if (g == 0) {
+        msh[wave][c16] = ref;
+        lsh[wave][c16] = l;
+    }
+    __syncthreads();
+    {
+        const float top = fmaxf(fmaxf(msh[0][c16], msh[1][c16]), fmaxf(msh[2][c16], msh[3][c16]));
+        const float w = ref_weight(ref, top, a.c);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < DJ; j += 4)
+                *reinterpret_cast<float4*>(osh + (wave * 16 + c16) * OS + DJ * (4 * g + i) + j) =
+                    make_float4(o[j][i] * w, o[j + 1][i] * w, o[j + 2][i] * w, o[j + 3][i] * w);
+    }
+    __syncthreads();
+    // 16 threads per row, DJ values each
+    const int row = threadIdx.x >> 4, d0 = DJ * (threadIdx.x & 15);
+    if (tile * 16 + row >= rows) return;
+    const float top = fmaxf(fmaxf(msh[0][row], msh[1][row]), fmaxf(msh[2][row], msh[3][row]));
+    float sum = 0.0f, v[DJ];
+#pragma unroll
+    for (int j = 0; j < DJ; j++) v[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        sum = sum + lsh[w][row] * ref_weight(msh[w][row], top, a.c);
+#pragma unroll
+        for (int j = 0; j < DJ; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(osh + (w * 16 + row) * OS + d0 + j);
+            v[j] += x.x;
+            v[j + 1] += x.y;
+            v[j + 2] += x.z;
+            v[j + 3] += x.w;
+        }
+    }
+    const int orow = tile * 16 + row, otok = q.start + orow / p.G, oh = kvh * p.G + orow % p.G;
+    if (a.splits > 1) {
+        const size_t at = ((size_t)split * p.n_tokens + otok) * p.nq + oh;
+        float* po = a.part_o + at * HD + d0;
+#pragma unroll
+        for (int j = 0; j < DJ; j += 4) *reinterpret_cast<float4*>(po + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        if (d0 == 0) a.part_ml[at] = make_float2(top, sum);
+        return;
+    }
+    uint16_t* dst = a.out + (size_t)otok * a.out_stride + (size_t)oh * HD + d0;
+#pragma unroll
+    for (int j = 0; j < DJ; j += 2)
+        *reinterpret_cast<uint32_t*>(dst + j) = pack16<T>(row_result(v[j], top, sum), row_result(v[j + 1], top, sum));
+    if (a.lse && d0 == 0) a.lse[(size_t)otok * p.nq + oh] = row_lse<T>(top, sum, a.scale);
+}
+
+// Joins the splits of one row: a wave per row.
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
+    constexpr int DL = HD / 64;
+    const Paged& p = a.p;
+    const int lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n_rows = (long long)p.n_tokens * p.nq;
+    if (row >= n_rows) return;
+    const int t = (int)(row / p.nq), h = (int)(row % p.nq);
+    const int r = find_req(p, t, lane);
+    if (r >= p.n_req) return;
+    const Req q = req_of(p, r);
+    const int i = t - q.start, n = min(q.n, p.max_q);
+    if (i < 0 || i >= n) return;
+    const int tile = (i * p.G + h % p.G) / 16;
+    const int kend = min(q.base + min(tile * 16 + 15, n * p.G - 1) / p.G + 1, p.limit);
+    const int ns = max((kend + a.split_keys - 1) / a.split_keys, 1);
+    float top = -INFINITY;
+    for (int s = lane; s < ns; s += 64) top = fmaxf(top, a.part_ml[s * n_rows + row].x);
+    top = wave_max(top);
+    float sum = 0.0f, v[DL];
+#pragma unroll
+    for (int d = 0; d < DL; d++) v[d] = 0.0f;
+    for (int s = 0; s < ns; s++) {
+        const float2 ml = a.part_ml[s * n_rows + row];
+        const float w = ref_weight(ml.x, top, a.c);
+        sum = sum + ml.y * w;
+        const float* po = a.part_o + (s * n_rows + row) * HD + DL * lane;
+#pragma unroll
+        for (int d = 0; d < DL; d++) v[d] = v[d] + po[d] * w;
+    }
+    uint16_t* dst = a.out + (size_t)t * a.out_stride + (size_t)h * HD + DL * lane;
+#pragma unroll
+    for (int d = 0; d < DL; d++) dst[d] = bits16<T>(row_result(v[d], top, sum));
+    if (a.lse && lane == 0) a.lse[row] = row_lse<T>(top, sum, a.scale);
+}
+
+// ---- received weight ---------------------------------------------------------------
+//
+// A wave owns 16 keys of one KV head, whose rows stay in registers as the matrix
+// operand, and goes over the query rows that see them, 16 at a time; nobody else
+// adds to those keys, so the sums have one order.
+struct MassArgs {
+    Paged p;
+    const uint16_t* q;
+    long long q_stride;
+    float scale;
+    const float* lse;
+};
+
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
+    constexpr int DS = HD / 32;
+    const Paged& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int g = lane >> 4, c16 = lane & 15;
+    const int r = blockIdx.z, kvh = blockIdx.y;
+    const Req q = req_of(p, r);
+    const int n = min(q.n, p.max_q), rows = n * p.G;
+    const int kend = min(q.base + n, p.limit);
+    const int kb = 64 * blockIdx.x + 16 * wave;
+    if (rows == 0 || kb >= kend) return;
+    const int pg = p.table[(size_t)r * p.max_pages + (kb >> p.shift)];
+    if ((unsigned)pg >= (unsigned)p.n_pages) return;
+    const size_t row = (((size_t)pg * p.nkv + kvh) << p.shift) + (kb & ((1 << p.shift) - 1));
+    u32x4_t kf[DS];
+#pragma unroll
+    for (int s = 0; s < DS; s++) kf[s] = *reinterpret_cast<const u32x4_t*>(p.kp + (row + c16) * HD + 32 * s + 8 * g);
+    float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
+    const int r0 = max(kb - q.base, 0) * p.G;              // the first row that sees key kb
+    for (int t0 = r0 & ~15; t0 < rows; t0 += 16) {
+        const int R = t0 + c16, Rc = min(R, rows - 1), i = Rc / p.G;
+        const int tok = q.start + i, h = kvh * p.G + Rc % p.G;
+        const uint16_t* qr = a.q + (size_t)tok * a.q_stride + (size_t)h * HD + 8 * g;
+        float4_t s = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DS; d++) s = mfma16(T(), kf[d], *reinterpret_cast<const u32x4_t*>(qr + 32 * d), s);
+        const float ls = a.lse[(size_t)tok * p.nq + h];
+        const int vis = R < rows && ls != -INFINITY ? min(q.base + i + 1, p.limit) : 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale, -ls) * kLog2e);
+            sum[e] = sum[e] + (kb + 4 * g + e < vis ? w : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] = row_sum16(sum[e]);
+    if (c16 < 4 && kb + 4 * g + c16 < kend) {
+        const float add = c16 == 0 ? sum[0] : c16 == 1 ? sum[1] : c16 == 2 ? sum[2] : sum[3];
+        p.mass[row + 4 * g + c16] += add;
+    }
+}
+
+// ---- eviction -------------------------------------------------------------------------
+
+struct EvictArgs {
+    Paged p;
+    int budget, sink, recent;
+    float* mass_out;
+    int* pos_out;
+    int* count;                // [n_req * nkv]: rows that move
+    int* from;                 // [n_req * nkv][most]: cache rows, in pairs
+    int* to;
+    int most, hd;
+};
+
+// Order of a mass: larger is larger, zeros alike, a NaN the least number.
+__device__ __forceinline__ uint32_t mass_key(float m) {
+    if (m != m) return 0u;
+    const uint32_t u = __float_as_uint(m == 0.0f ? 0.0f : m);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+constexpr int kSelThreads = 1024;
+
+// One workgroup per (request, KV head): the key of the last row that stays by a
+// radix selection over 4 x 8 bits, then one ordered pass that counts ties and
+// pairs the gaps with the rows that fill them.
+__global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
+    __shared__ int hist[256];
+    __shared__ int wsum[kSelThreads / 64][3];
+    __shared__ int s_newest, s_digit, s_left;
+    const Paged& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x, r = blockIdx.y, item = r * p.nkv + h;
+    const int n = min(max(p.kv_len[r], 0), p.limit);
+    if (n <= a.budget) {
+        if (tid == 0) a.count[item] = 0;
+        for (int j = tid; j < n; j += kSelThreads) {
+            const long long at = pool_row(p, r, h, j);
+            if (at < 0) continue;
+            a.mass_out[at] = p.mass[at];
+            a.pos_out[at] = p.pos[at];
+        }
+        return;
+    }
+    if (tid == 0) s_newest = -1;
+    __syncthreads();
+    int newest = -1;
+    for (int j = tid; j < n; j += kSelThreads) {
+        const long long at = pool_row(p, r, h, j);
+        if (at >= 0) newest = max(newest, p.pos[at]);
+    }
+    atomicMax(&s_newest, newest);
+    __syncthreads();
+    newest = s_newest;
+    auto key_of = [&](int j) -> uint32_t {
+        const long long at = pool_row(p, r, h, j);
+        if (at < 0) return 0u;
+        const int pos = p.pos[at];
+        if (pos < a.sink || (long long)pos > (long long)newest - a.recent) return 0xffffffffu;
+        return mass_key(p.mass[at]);
+    };
+    uint32_t prefix = 0;
+    int left = a.budget;                  // rows still wanted among those with this prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < n; j += kSelThreads) {
+            const uint32_t k = key_of(j);
+            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int d = 255, above = 0;
+            while (d > 0 && above + hist[d] < left) above += hist[d--];
+            s_digit = d;
+            s_left = left - above;
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_digit << shift;
+        left = s_left;
+        __syncthreads();
+    }
+    // in order: how many ties, gaps and fillers come before each row
+    int ties = 0, gaps = 0, fill = 0;
+    for (int j0 = 0; j0 < n; j0 += kSelThreads) {
+        const int j = j0 + tid;
+        const uint32_t k = j < n ? key_of(j) : 0u;
+        const bool tie = j < n && k == prefix;
+        const unsigned long long bt = __ballot(tie), below = (1ull << lane) - 1;
+        if (lane == 0) wsum[wave][0] = __popcll(bt);
+        __syncthreads();
+        int before = ties, all = 0;
+        for (int w = 0; w < kSelThreads / 64; w++) {
+            if (w < wave) before += wsum[w][0];
+            all += wsum[w][0];
+        }
+        ties += all;
+        const bool stay = j < n && (k > prefix || (tie && before + __popcll(bt & below) < left));
+        const bool gap = j < a.budget && !stay, filler = j >= a.budget && stay;
+        const unsigned long long bg = __ballot(gap), bf = __ballot(filler);
+        if (lane == 0) {
+            wsum[wave][1] = __popcll(bg);
+            wsum[wave][2] = __popcll(bf);
+        }
+        __syncthreads();
+        int g0 = gaps, f0 = fill, ga = 0, fa = 0;
+        for (int w = 0; w < kSelThreads / 64; w++) {
+            if (w < wave) {
+                g0 += wsum[w][1];
+                f0 += wsum[w][2];
+            }
+            ga += wsum[w][1];
+            fa += wsum[w][2];
+        }
+        gaps += ga;
+        fill += fa;
+        const size_t list = (size_t)item * a.most;
+        if (gap) a.to[list + g0 + __popcll(bg & below)] = j;
+        if (filler) a.from[list + f0 + __popcll(bf & below)] = j;
+        if (stay && j < a.budget) {
+            const long long at = pool_row(p, r, h, j);
+            if (at >= 0) {
+                a.mass_out[at] = p.mass[at];
+                a.pos_out[at] = p.pos[at];
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) a.count[item] = fill;
+}
+
+// Moves rows; sources lie behind the budget and targets before it, so no order
+// is needed.  16 bytes per thread, hd / 8 threads per row.
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+    const Paged& p = a.p;
+    const int h = blockIdx.y, r = blockIdx.z, item = r * p.nkv + h;
+    const int per = a.hd / 8, rows = 256 / per, c = threadIdx.x % per;
+    const int count = a.count[item];
+    const size_t list = (size_t)item * a.most;
+    for (int m = blockIdx.x * rows + threadIdx.x / per; m < count; m += gridDim.x * rows) {
+        const long long src = pool_row(p, r, h, a.from[list + m]), dst = pool_row(p, r, h, a.to[list + m]);
+        if (src < 0 || dst < 0) continue;
+        const uint4 k = *reinterpret_cast<const uint4*>(p.kp + src * a.hd + 8 * c);
+        const uint4 v = *reinterpret_cast<const uint4*>(p.vp + src * a.hd + 8 * c);
+        *reinterpret_cast<uint4*>(p.kp + dst * a.hd + 8 * c) = k;
+        *reinterpret_cast<uint4*>(p.vp + dst * a.hd + 8 * c) = v;
+        if (c == 0) {
+            a.mass_out[dst] = p.mass[src];
+            a.pos_out[dst] = p.pos[src];
+        }
+    }
+}
+
+// ---- shapes -----------------------------------------------------------------------------
+
+struct Splits {
+    int n, keys;
+};
+// Enough workgroups for the chip, but splits of at least 256 keys.
+Splits attn_splits(const Paged& p) {
+    const long long blocks = (long long)p.n_req * p.nkv * cdiv((long long)p.max_q * p.G, 16);
+    long long want = cdiv(1024, blocks > 0 ? blocks : 1);
+    const long long most = cdiv(p.limit > 0 ? p.limit : 1, 256);
+    if (want > most) want = most;
+    Splits s;
+    s.keys = cdiv(cdiv(p.limit > 0 ? p.limit : 1, want), 128) * 128;
+    s.n = cdiv(p.limit > 0 ? p.limit : 1, s.keys);
+    return s;
+}
+
+size_t attn_rows(const Paged& p) { return (size_t)p.n_tokens * p.nq; }
+
+}  // namespace
+
+#define MDX_PAGED_HD(FN, ...)                                                                     \
+    (c->type == MDX_TYPE_F16                                                                      \
+         ? (c->head_dim == 64 ? FN<64, _Float16>(__VA_ARGS__)                                     \
+                              : c->head_dim == 128 ? FN<128, _Float16>(__VA_ARGS__) : FN<256, _Float16>(__VA_ARGS__)) \
+         : (c->head_dim == 64 ? FN<64, __bf16>(__VA_ARGS__)                                       \
+                              : c->head_dim == 128 ? FN<128, __bf16>(__VA_ARGS__) : FN<256, __bf16>(__VA_ARGS__)))
+
+namespace {
+
+template <int HD, class T>
+void append_launch(const AppendArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((k_paged_append<HD, T>), dim3(a.p.n_tokens), dim3(256), 0, s, a);
+}
+
+template <int HD, class T>
+void attn_launch(const AttnArgs& a, int tiles, hipStream_t s) {
+    hipLaunchKernelGGL((k_paged_attn<HD, T>), dim3(a.splits, a.p.nkv * tiles, a.p.n_req), dim3(256), 0, s, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((k_paged_join<HD, T>), dim3(cdiv((long long)attn_rows(a.p), 4)), dim3(256), 0, s, a);
+}
+
+template <int HD, class T>
+void mass_launch(const MassArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((k_paged_mass<HD, T>), dim3(cdiv(a.p.limit, 64), a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdx_launch_paged_append(const MdxPagedCache* c, const MdxPagedBatch* b, const float* qkv, long long qkv_stride,
+                            const int* positions, const float* q_norm, const float* k_norm, float eps,
+                            const float* cos_t, const float* sin_t, int max_pos, int rope_style, void* q_out,
+                            long long q_stride, void* stream) {
+    AppendArgs a = {};
+    a.p = paged(c, b);
+    a.qkv = qkv;
+    a.qkv_stride = qkv_stride;
+    a.positions = positions;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = eps;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.max_pos = max_pos;
+    a.style = rope_style;
+    a.q_out = (uint16_t*)q_out;
+    a.q_stride = q_stride;
+    MDX_PAGED_HD(append_launch, a, (hipStream_t)stream);
+    return mdxrt_launched("mdx_paged_append");
+}
+
+size_t mdx_paged_attn_scratch(const MdxPagedCache* c, const MdxPagedBatch* b) {
+    const Paged p = paged(c, b);
+    const Splits s = attn_splits(p);
+    return s.n > 1 ? (size_t)s.n * attn_rows(p) * ((size_t)c->head_dim * 4 + 8) : 0;
+}
+
+int mdx_launch_paged_attn(const MdxPagedCache* c, const MdxPagedBatch* b, const void* q, long long q_stride,
+                          float scale, void* out, long long out_stride, float* lse, void* scratch, void* stream) {
+    AttnArgs a = {};
+    a.p = paged(c, b);
+    if (a.p.max_q == 0) return 0;
+    const Splits s = attn_splits(a.p);
+    a.q = (const uint16_t*)q;
+    a.q_stride = q_stride;
+    a.scale = scale;
+    a.c = scale * kLog2e;
+    a.out = (uint16_t*)out;
+    a.out_stride = out_stride;
+    a.lse = lse;
+    a.splits = s.n;
+    a.split_keys = s.keys;
+    a.part_o = (float*)scratch;
+    a.part_ml = (float2*)((float*)scratch + (s.n > 1 ? (size_t)s.n * attn_rows(a.p) * c->head_dim : 0));
+    const long long tiles = cdiv((long long)a.p.max_q * a.p.G, 16);
+    if (tiles * a.p.nkv > 65535) return mdxrt_refuse(-1, "mdx_paged_attention: max_q_len is too large");
+    MDX_PAGED_HD(attn_launch, a, (int)tiles, (hipStream_t)stream);
+    return mdxrt_launched("mdx_paged_attention");
+}
+
+size_t mdx_paged_mass_scratch(const MdxPagedCache* c, const MdxPagedBatch* b) {
+    (void)c;
+    (void)b;
+    return 0;
+}
+
+int mdx_launch_paged_mass(const MdxPagedCache* c, const MdxPagedBatch* b, const void* q, long long q_stride,
+                          float scale, const float* lse, void* scratch, void* stream) {
+    (void)scratch;
+    MassArgs a = {};
+    a.p = paged(c, b);
+    if (a.p.max_q == 0 || a.p.limit == 0) return 0;
+    a.q = (const uint16_t*)q;
+    a.q_stride = q_stride;
+    a.scale = scale;
+    a.lse = lse;
+    MDX_PAGED_HD(mass_launch, a, (hipStream_t)stream);
+    return mdxrt_launched("mdx_paged_mass");
+}
+
+static int evict_most(const Paged& p, int budget) {
+    return p.limit <= budget ? 0 : (p.limit - budget < budget ? p.limit - budget : budget);
+}
+
+size_t mdx_paged_evict_scratch(const MdxPagedCache* c, const MdxPagedBatch* b, int budget) {
+    const Paged p = paged(c, b);
+    return (size_t)p.n_req * p.nkv * 4 * (1 + 2 * (size_t)evict_most(p, budget));
+}
+
+int mdx_launch_paged_evict(const MdxPagedCache* c, const MdxPagedBatch* b, int budget, int sink, int recent,
+                           float* mass_out, int* pos_out, void* scratch, void* stream) {
+    EvictArgs a = {};
+    a.p = paged(c, b);
+    a.budget = budget;
+    a.sink = sink;
+    a.recent = recent;
+    a.mass_out = mass_out;
+    a.pos_out = pos_out;
+    a.most = evict_most(a.p, budget);
+    a.hd = c->head_dim;
+    const size_t items = (size_t)a.p.n_req * a.p.nkv;
+    a.count = (int*)scratch;
+    a.from = a.count + items;
+    a.to = a.from + items * a.most;
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(k_evict_select, dim3(a.p.nkv, a.p.n_req), dim3(kSelThreads), 0, s, a);
+    if (a.most > 0) {
+        const int rows = 256 / (a.hd / 8);
+        const int blocks = cdiv(a.most, rows) < 32 ? cdiv(a.most, rows) : 32;
+        hipLaunchKernelGGL(k_evict_move, dim3(blocks, a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
+    }
+    return mdxrt_launched("mdx_paged_evict");
+}
+
+}  // extern "C"

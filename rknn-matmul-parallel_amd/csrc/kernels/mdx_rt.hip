@@ -82,6 +82,16 @@ int mdxrt_device_count(void) {
 
 const char* mdxrt_last_error(void) { return g_last_error; }
 
+int mdxrt_refuse(int rc, const char* message) {
+    std::snprintf(g_last_error, sizeof g_last_error, "%s", message);
+    return rc;
+}
+
+int mdxrt_launched(const char* what) {
+    MDX_CHECK(hipGetLastError(), what);
+    return 0;
+}
+
 int mdxrt_malloc(void** p, size_t bytes) {
     *p = nullptr;
     MDX_CHECK(hipMalloc(p, bytes ? bytes : 256), "hipMalloc");

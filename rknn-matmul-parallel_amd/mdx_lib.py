@@ -67,6 +67,24 @@ class RmpConfig(C.Structure):
                 ("layout", C.c_int), ("n_workers", C.c_int)]
 
 
+class PagedCache(C.Structure):
+    """Mirror of MdxPagedCache (include/mdx_ext.h)."""
+    _fields_ = [("type", C.c_int), ("num_q_heads", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("n_pages", C.c_int), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p),
+                ("mass", C.c_void_p), ("pos", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """Mirror of MdxPagedBatch (include/mdx_ext.h)."""
+    _fields_ = [("n_req", C.c_int), ("n_tokens", C.c_int), ("max_q_len", C.c_int), ("max_kv_len", C.c_int),
+                ("max_pages", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("block_table", C.c_void_p)]
+
+
+_PC = C.POINTER(PagedCache)
+_PB = C.POINTER(PagedBatch)
+
+
 def qwen3_0_6b_config(**overrides) -> MatmulDecoderConfig:
     """matmul_decoder_config_qwen3_0_6b() with field overrides."""
     c = MatmulDecoderConfig(
@@ -139,6 +157,15 @@ def lib() -> C.CDLL:
             "mdx_time_gemv": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _F]),
             "mdx_sample_topk_noalloc": (C.c_int, [P, C.c_int, C.c_float, C.c_int, C.c_float, C.c_float,
                                                   P, P, P, P]),
+            "mdx_paged_append": (C.c_int, [_PC, _PB, P, C.c_longlong, P, P, P, C.c_float, P, P, C.c_int, C.c_int,
+                                           P, C.c_longlong, P]),
+            "mdx_paged_attention_workspace": (C.c_size_t, [_PC, _PB]),
+            "mdx_paged_attention": (C.c_int, [_PC, _PB, P, C.c_longlong, C.c_float, P, C.c_longlong, P, P,
+                                              C.c_size_t, P]),
+            "mdx_paged_mass_workspace": (C.c_size_t, [_PC, _PB]),
+            "mdx_paged_mass": (C.c_int, [_PC, _PB, P, C.c_longlong, C.c_float, P, P, C.c_size_t, P]),
+            "mdx_paged_evict_workspace": (C.c_size_t, [_PC, _PB, C.c_int]),
+            "mdx_paged_evict": (C.c_int, [_PC, _PB, C.c_int, C.c_int, C.c_int, P, P, P, C.c_size_t, P]),
             "mdx_device_malloc": (C.c_int, [C.POINTER(C.c_void_p), C.c_size_t]),
             "mdx_device_free": (C.c_int, [P]),
             "mdx_memcpy_h2d": (C.c_int, [P, P, C.c_size_t]),
@@ -352,6 +379,75 @@ def sample(logits, top_k=1, temperature=1.0, top_p=1.0, u=0.0, repeat_tokens=(),
     _check(lib().mdx_debug_sample(_p(x, _F), x.size, C.byref(p), float(u), _p(out, _I), _p(idx, _I),
                                   _p(val, _F)), "sample")
     return int(out[0]), idx, val, int(out[1])
+
+
+# ---- many requests over a paged cache (device pointers) ------------------------------
+#
+# Device arrays are given as addresses (int or c_void_p) or as objects with a
+# data_ptr() (a torch tensor: import torch before this library is loaded, so
+# that both use one HIP runtime).  The calls enqueue and return; what they
+# mean, and what they refuse, stands in mdx_ext.h.
+
+PAGED_TYPES = {"fp16": 0, "bf16": 1}
+
+
+def _dev(a):
+    return a.data_ptr() if hasattr(a, "data_ptr") else a
+
+
+def paged_cache(dtype, num_q_heads, num_kv_heads, head_dim, page_size, n_pages, k_pages, v_pages, mass=None,
+                pos=None) -> PagedCache:
+    return PagedCache(PAGED_TYPES[dtype] if isinstance(dtype, str) else dtype, num_q_heads, num_kv_heads, head_dim,
+                      page_size, n_pages, _dev(k_pages), _dev(v_pages), _dev(mass), _dev(pos))
+
+
+def paged_batch(n_req, n_tokens, max_q_len, max_kv_len, max_pages, q_start, kv_len, block_table) -> PagedBatch:
+    return PagedBatch(n_req, n_tokens, max_q_len, max_kv_len, max_pages, _dev(q_start), _dev(kv_len),
+                      _dev(block_table))
+
+
+def paged_append(cache, batch, qkv, positions, cos, sin, max_pos, q_out, q_norm=None, k_norm=None, eps=1e-6,
+                 rope_style=0, qkv_stride=None, q_stride=None, stream=None) -> None:
+    """mdx_paged_append; strides default to rows without gaps."""
+    qd, kvd = cache.num_q_heads * cache.head_dim, cache.num_kv_heads * cache.head_dim
+    _check(lib().mdx_paged_append(cache, batch, _dev(qkv), qd + 2 * kvd if qkv_stride is None else qkv_stride,
+                                  _dev(positions), _dev(q_norm), _dev(k_norm), eps, _dev(cos), _dev(sin), max_pos,
+                                  rope_style, _dev(q_out), qd if q_stride is None else q_stride, stream), "paged_append")
+
+
+def paged_attention_workspace(cache, batch) -> int:
+    return lib().mdx_paged_attention_workspace(cache, batch)
+
+
+def paged_attention(cache, batch, q, out, workspace, workspace_bytes, lse=None, scale=0.0, q_stride=None,
+                    out_stride=None, stream=None) -> None:
+    """mdx_paged_attention; strides default to rows without gaps."""
+    qd = cache.num_q_heads * cache.head_dim
+    _check(lib().mdx_paged_attention(cache, batch, _dev(q), qd if q_stride is None else q_stride, scale, _dev(out),
+                                     qd if out_stride is None else out_stride, _dev(lse), _dev(workspace),
+                                     workspace_bytes, stream), "paged_attention")
+
+
+def paged_mass_workspace(cache, batch) -> int:
+    return lib().mdx_paged_mass_workspace(cache, batch)
+
+
+def paged_mass(cache, batch, q, lse, workspace, workspace_bytes, scale=0.0, q_stride=None, stream=None) -> None:
+    """mdx_paged_mass; the stride defaults to rows without gaps."""
+    qd = cache.num_q_heads * cache.head_dim
+    _check(lib().mdx_paged_mass(cache, batch, _dev(q), qd if q_stride is None else q_stride, scale, _dev(lse),
+                                _dev(workspace), workspace_bytes, stream), "paged_mass")
+
+
+def paged_evict_workspace(cache, batch, budget) -> int:
+    return lib().mdx_paged_evict_workspace(cache, batch, budget)
+
+
+def paged_evict(cache, batch, budget, sink, recent, mass_out, pos_out, workspace, workspace_bytes,
+                stream=None) -> None:
+    """mdx_paged_evict; mass_out / pos_out: the cache's own arrays or others of their size."""
+    _check(lib().mdx_paged_evict(cache, batch, budget, sink, recent, _dev(mass_out), _dev(pos_out), _dev(workspace),
+                                 workspace_bytes, stream), "paged_evict")
 
 
 # ---- decoder ---------------------------------------------------------------------
