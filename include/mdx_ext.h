@@ -286,7 +286,8 @@ typedef struct {
     int n_pages;            /* pages in the pool */
     void* k_pages;          /* [n_pages][num_kv_heads][page_size][head_dim], 16-byte aligned */
     void* v_pages;
-    float* mass;            /* [n_pages][num_kv_heads][page_size]: weight received (NULL: not kept) */
+    float* mass;            /* [n_pages][num_kv_heads][page_size], 16-byte aligned: weight received
+                               (NULL: not kept) */
     int* pos;               /* the same: the row's position in its request (NULL: not kept) */
 } MdxPagedCache;
 

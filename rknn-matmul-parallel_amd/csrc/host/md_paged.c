@@ -27,7 +27,7 @@ static int check_cache(const MdxPagedCache* c, const char* fn) {
     REFUSE_IF(c->num_q_heads > 65535, "too many heads");
     REFUSE_IF(c->n_pages < 1 || !c->k_pages || !c->v_pages, "no pages");
     REFUSE_IF(misaligned(c->k_pages, 16) || misaligned(c->v_pages, 16), "pages have to be 16-byte aligned");
-    REFUSE_IF(misaligned(c->mass, 4) || misaligned(c->pos, 4), "mass and pos have to be 4-byte aligned");
+    REFUSE_IF(misaligned(c->mass, 16) || misaligned(c->pos, 16), "mass and pos have to be 16-byte aligned");
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return refuse(MATMUL_DECODER_ERR_UNSUPPORTED, fn, "head_dim has to be 64, 128 or 256");
     if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))

@@ -23,6 +23,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+// a / b up to a multiple of 4
+__device__ __forceinline__ int cdiv4(int a, int b) { return ((a - 1) / b / 4 + 1) * 4; }
 
 // The cache and the batch as the kernels take them.
 struct Paged {
@@ -591,6 +593,7 @@ struct EvictArgs {
     int* from;                 // [n_req * nkv][most]: cache rows, in pairs
     int* to;
     int most, hd;
+    int move_here;             // the selecting workgroup also moves the rows
 };
 
 // Order of a mass: larger is larger, zeros alike, a NaN the least number.
@@ -599,126 +602,41 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
     const uint32_t u = __float_as_uint(m == 0.0f ? 0.0f : m);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+constexpr uint32_t kProtected = 0xffffffffu;      // above the key of any mass
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr int kSelBins = 2048;
+constexpr int kSelMoves = 64;      // moves that the selecting workgroup makes itself
 
-// One workgroup per (request, KV head): the key of the last row that stays by a
-// radix selection over 4 x 8 bits, then one ordered pass that counts ties and
-// pairs the gaps with the rows that fill them.
-__global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
-    __shared__ int hist[256];
-    __shared__ int wsum[kSelThreads / 64][3];
-    __shared__ int s_newest, s_digit, s_left;
-    const Paged& p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = blockIdx.x, r = blockIdx.y, item = r * p.nkv + h;
-    const int n = min(max(p.kv_len[r], 0), p.limit);
-    if (n <= a.budget) {
-        if (tid == 0) a.count[item] = 0;
-        for (int j = tid; j < n; j += kSelThreads) {
-            const long long at = pool_row(p, r, h, j);
-            if (at < 0) continue;
-            a.mass_out[at] = p.mass[at];
-            a.pos_out[at] = p.pos[at];
-        }
-        return;
+// Sum over the threads before this one, and over all; `sums` is scratch.
+__device__ __forceinline__ int sel_scan(int v, int* sums, int lane, int wave, int* total) {
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(incl, o, kWave);
+        if (lane >= o) incl += y;
     }
-    if (tid == 0) s_newest = -1;
     __syncthreads();
-    int newest = -1;
-    for (int j = tid; j < n; j += kSelThreads) {
-        const long long at = pool_row(p, r, h, j);
-        if (at >= 0) newest = max(newest, p.pos[at]);
-    }
-    atomicMax(&s_newest, newest);
+    if (lane == 63) sums[wave] = incl;
     __syncthreads();
-    newest = s_newest;
-    auto key_of = [&](int j) -> uint32_t {
-        const long long at = pool_row(p, r, h, j);
-        if (at < 0) return 0u;
-        const int pos = p.pos[at];
-        if (pos < a.sink || (long long)pos > (long long)newest - a.recent) return 0xffffffffu;
-        return mass_key(p.mass[at]);
-    };
-    uint32_t prefix = 0;
-    int left = a.budget;                  // rows still wanted among those with this prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += kSelThreads) {
-            const uint32_t k = key_of(j);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int d = 255, above = 0;
-            while (d > 0 && above + hist[d] < left) above += hist[d--];
-            s_digit = d;
-            s_left = left - above;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)s_digit << shift;
-        left = s_left;
-        __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; w++) {
+        const int s = sums[w];
+        before += w < wave ? s : 0;
+        all += s;
     }
-    // in order: how many ties, gaps and fillers come before each row
-    int ties = 0, gaps = 0, fill = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        const uint32_t k = j < n ? key_of(j) : 0u;
-        const bool tie = j < n && k == prefix;
-        const unsigned long long bt = __ballot(tie), below = (1ull << lane) - 1;
-        if (lane == 0) wsum[wave][0] = __popcll(bt);
-        __syncthreads();
-        int before = ties, all = 0;
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w < wave) before += wsum[w][0];
-            all += wsum[w][0];
-        }
-        ties += all;
-        const bool stay = j < n && (k > prefix || (tie && before + __popcll(bt & below) < left));
-        const bool gap = j < a.budget && !stay, filler = j >= a.budget && stay;
-        const unsigned long long bg = __ballot(gap), bf = __ballot(filler);
-        if (lane == 0) {
-            wsum[wave][1] = __popcll(bg);
-            wsum[wave][2] = __popcll(bf);
-        }
-        __syncthreads();
-        int g0 = gaps, f0 = fill, ga = 0, fa = 0;
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w < wave) {
-                g0 += wsum[w][1];
-                f0 += wsum[w][2];
-            }
-            ga += wsum[w][1];
-            fa += wsum[w][2];
-        }
-        gaps += ga;
-        fill += fa;
-        const size_t list = (size_t)item * a.most;
-        if (gap) a.to[list + g0 + __popcll(bg & below)] = j;
-        if (filler) a.from[list + f0 + __popcll(bf & below)] = j;
-        if (stay && j < a.budget) {
-            const long long at = pool_row(p, r, h, j);
-            if (at >= 0) {
-                a.mass_out[at] = p.mass[at];
-                a.pos_out[at] = p.pos[at];
-            }
-        }
-        __syncthreads();
-    }
-    if (tid == 0) a.count[item] = fill;
+    *total = all;
+    return before + incl - v;
 }
 
-// Moves rows; sources lie behind the budget and targets before it, so no order
-// is needed.  16 bytes per thread, hd / 8 threads per row.
-__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+// A thread's row moves; sources lie behind the budget and targets before it, so
+// no order is needed.  16 bytes per thread, hd / 8 threads per row.
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, int count, int first, int step) {
     const Paged& p = a.p;
-    const int h = blockIdx.y, r = blockIdx.z, item = r * p.nkv + h;
-    const int per = a.hd / 8, rows = 256 / per, c = threadIdx.x % per;
-    const int count = a.count[item];
-    const size_t list = (size_t)item * a.most;
-    for (int m = blockIdx.x * rows + threadIdx.x / per; m < count; m += gridDim.x * rows) {
+    const int per = a.hd / 8, c = threadIdx.x % per;
+    const size_t list = (size_t)(r * p.nkv + h) * a.most;
+    for (int m = first + threadIdx.x / per; m < count; m += step) {
         const long long src = pool_row(p, r, h, a.from[list + m]), dst = pool_row(p, r, h, a.to[list + m]);
         if (src < 0 || dst < 0) continue;
         const uint4 k = *reinterpret_cast<const uint4*>(p.kp + src * a.hd + 8 * c);
@@ -730,6 +648,169 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
             a.pos_out[dst] = p.pos[src];
         }
     }
+}
+
+// One workgroup per (request, KV head).  A thread owns C consecutive rows (a
+// multiple of 4, so that four masses or positions are one load) and keeps their
+// keys in registers; C = 0: as many rows as it takes, read again in each pass.
+// The key of the last row that stays comes from a radix selection of 11, 11 and
+// 10 bits with histograms in LDS (the first digit is a mass's exponent and two
+// bits: 8 bits would put most rows into a few counters), then three scans over
+// the threads number the ties, the gaps and the rows that fill them.
+template <int C>
+__global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
+    __shared__ int hist[kSelBins];
+    __shared__ int sums[kSelWaves];
+    __shared__ int s_newest, s_digit, s_left;
+    const Paged& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x, r = blockIdx.y, item = r * p.nkv + h;
+    const int n = min(max(p.kv_len[r], 0), p.limit);
+    const bool copy = a.mass_out != p.mass || a.pos_out != p.pos;
+    if (n <= a.budget) {
+        if (tid == 0) a.count[item] = 0;
+        for (int j = tid; copy && j < n; j += kSelThreads) {
+            const long long at = pool_row(p, r, h, j);
+            if (at < 0) continue;
+            a.mass_out[at] = p.mass[at];
+            a.pos_out[at] = p.pos[at];
+        }
+        return;
+    }
+    const int per = C ? C : cdiv4(n, kSelThreads);
+    const int j0 = tid * per, j1 = min(n, j0 + per);
+
+    // rows j..j+3 (j a multiple of 4): their place in the pool, or -1
+    auto place = [&](int j) -> long long { return j < j1 ? pool_row(p, r, h, j) : -1; };
+    if (tid == 0) s_newest = -1;
+    __syncthreads();
+    uint32_t key[C ? C : 1];
+    {
+        int newest = -1;
+        auto positions = [&](int j) __attribute__((always_inline)) {
+            const long long at = place(j);
+            int4 q = make_int4(-1, -1, -1, -1);
+            if (at >= 0) q = *reinterpret_cast<const int4*>(p.pos + at);
+            newest = max(newest, max(max(q.x, j + 1 < j1 ? q.y : -1), max(j + 2 < j1 ? q.z : -1, j + 3 < j1 ? q.w : -1)));
+        };
+        if constexpr (C != 0) {
+#pragma unroll
+            for (int c = 0; c < C; c += 4) positions(j0 + c);
+        } else {
+            for (int j = j0; j < j1; j += 4) positions(j);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, kWave));
+        if (lane == 0) atomicMax(&s_newest, newest);
+    }
+    __syncthreads();
+    const long long recent = (long long)s_newest - a.recent;
+    auto keys4 = [&](int j, uint32_t (&k)[4]) __attribute__((always_inline)) {
+        const long long at = place(j);
+        k[0] = k[1] = k[2] = k[3] = 0u;
+        if (at < 0) return;
+        const float4 m = *reinterpret_cast<const float4*>(p.mass + at);
+        const int4 q = *reinterpret_cast<const int4*>(p.pos + at);
+        k[0] = q.x < a.sink || q.x > recent ? kProtected : mass_key(m.x);
+        k[1] = q.y < a.sink || q.y > recent ? kProtected : mass_key(m.y);
+        k[2] = q.z < a.sink || q.z > recent ? kProtected : mass_key(m.z);
+        k[3] = q.w < a.sink || q.w > recent ? kProtected : mass_key(m.w);
+    };
+    if constexpr (C != 0) {
+#pragma unroll
+        for (int c = 0; c < C; c += 4) {
+            uint32_t k[4];
+            keys4(j0 + c, k);
+#pragma unroll
+            for (int e = 0; e < 4; e++) key[c + e] = k[e];
+        }
+    }
+    // f(row, key) for this thread's rows in order
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (C != 0) {
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                if (j0 + c < j1) f(j0 + c, key[c]);
+        } else {
+            for (int j = j0; j < j1; j += 4) {
+                uint32_t k[4];
+                keys4(j, k);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (j + e < j1) f(j + e, k[e]);
+            }
+        }
+    };
+
+    int safe = 0, total;
+    each([&](int, uint32_t k) { safe += k == kProtected; });
+    sel_scan(safe, sums, lane, wave, &total);
+    // kth: the least key that stays; left: how many rows of that key stay
+    uint32_t kth = kProtected;
+    int left = a.budget;
+    if (total < a.budget) {
+        left = a.budget - total;
+        uint32_t prefix = 0;
+        int top = 32;                     // bits above `top` are known
+        while (top > 0) {
+            const int bits = top > 11 ? 11 : top, shift = top - bits;
+            for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
+            __syncthreads();
+            each([&](int, uint32_t k) {
+                if (k != kProtected && (top == 32 || (k >> top) == (prefix >> top)))
+                    atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+            });
+            __syncthreads();
+            // bins from the largest digit down, two per thread
+            const int b1 = kSelBins - 1 - 2 * tid, c1 = hist[b1], c0 = hist[b1 - 1];
+            int all;
+            const int above = sel_scan(c1 + c0, sums, lane, wave, &all);
+            if (above < left && above + c1 + c0 >= left) {
+                const bool second = above + c1 < left;
+                s_digit = second ? b1 - 1 : b1;
+                s_left = left - above - (second ? c1 : 0);
+            }
+            __syncthreads();
+            prefix |= (uint32_t)s_digit << shift;
+            left = s_left;
+            top = shift;
+        }
+        kth = prefix;
+    }
+    int ties = 0;
+    each([&](int, uint32_t k) { ties += k == kth; });
+    const int before = sel_scan(ties, sums, lane, wave, &total);
+    int tie = before, gaps = 0, fill = 0;
+    each([&](int j, uint32_t k) {
+        const bool stay = k > kth || (k == kth && tie++ < left);
+        gaps += !stay && j < a.budget;
+        fill += stay && j >= a.budget;
+    });
+    int moves;
+    int g = sel_scan(gaps, sums, lane, wave, &total), f = sel_scan(fill, sums, lane, wave, &moves);
+    const size_t list = (size_t)item * a.most;
+    tie = before;
+    each([&](int j, uint32_t k) {
+        const bool stay = k > kth || (k == kth && tie++ < left);
+        if (!stay && j < a.budget) a.to[list + g++] = j;
+        if (stay && j >= a.budget) a.from[list + f++] = j;
+        if (stay && j < a.budget && copy) {
+            const long long at = pool_row(p, r, h, j);
+            if (at >= 0) {
+                a.mass_out[at] = p.mass[at];
+                a.pos_out[at] = p.pos[at];
+            }
+        }
+    });
+    if (tid == 0) a.count[item] = moves;
+    if (!a.move_here) return;
+    __syncthreads();
+    move_rows(a, r, h, moves, 0, kSelThreads / (a.hd / 8));
+}
+
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+    const int h = blockIdx.y, r = blockIdx.z, rows = 256 / (a.hd / 8);
+    move_rows(a, r, h, a.count[r * a.p.nkv + h], blockIdx.x * rows, gridDim.x * rows);
 }
 
 // ---- shapes -----------------------------------------------------------------------------
@@ -879,11 +960,15 @@ int mdx_launch_paged_evict(const MdxPagedCache* c, const MdxPagedBatch* b, int b
     a.from = a.count + items;
     a.to = a.from + items * a.most;
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_evict_select, dim3(a.p.nkv, a.p.n_req), dim3(kSelThreads), 0, s, a);
-    if (a.most > 0) {
-        const int rows = 256 / (a.hd / 8);
-        const int blocks = cdiv(a.most, rows) < 32 ? cdiv(a.most, rows) : 32;
-        hipLaunchKernelGGL(k_evict_move, dim3(blocks, a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
+    a.move_here = a.most <= kSelMoves;
+    const dim3 grid(a.p.nkv, a.p.n_req), block(kSelThreads);
+    const int per = cdiv(a.p.limit, kSelThreads);
+    if (per <= 4) hipLaunchKernelGGL(k_evict_select<4>, grid, block, 0, s, a);
+    else if (per <= 16) hipLaunchKernelGGL(k_evict_select<16>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(k_evict_select<0>, grid, block, 0, s, a);
+    if (!a.move_here) {
+        const int rows = 256 / (a.hd / 8), need = cdiv(a.most, rows);
+        hipLaunchKernelGGL(k_evict_move, dim3(need < 64 ? need : 64, a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
     }
     return mdxrt_launched("mdx_paged_evict");
 }

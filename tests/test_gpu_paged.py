@@ -372,6 +372,16 @@ def test_evict_ties_and_odd_masses(mdx, gpu, what):
     _evict(mdx, w, 64, 3, 20, True)
 
 
+@pytest.mark.parametrize("kv,budget,recent", [([4096, 4097, 4100], 4000, 100), ([16384, 16383, 70], 64, 10), ([16385, 300], 5000, 700), ([40001, 2], 9, 0)])
+def test_evict_lengths_of_each_variant(mdx, gpu, kv, budget, recent):
+    """Rows per thread: 4, 16 and any number."""
+    rng = np.random.default_rng(kv[0])
+    w = World(rng, "fp16", 1, 1, 64, 64, [0] * len(kv), kv)
+    w.mass = np.round(8 * rng.random(w.mass.shape) ** 4, 2).astype(np.float32)
+    _positions(w, rng, True)
+    _evict(mdx, w, budget, 4, recent, True)
+
+
 def test_evict_takes_the_most_recent_by_position(mdx, gpu):
     """Positions far from the rows' numbers, at the ends of their type."""
     rng = np.random.default_rng(1)

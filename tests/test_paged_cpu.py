@@ -45,7 +45,8 @@ def _refused(mdx, call, c, b, rc, says, **k):
     (dict(page_size=8), -5, "page_size"), (dict(page_size=24), -5, "page_size"), (dict(page_size=2048), -5, "page_size"),
     (dict(page_size=0), -5, "page_size"), (dict(page_size=-16), -5, "page_size"),
     (dict(n_pages=0), -1, "no pages"), (dict(k_pages=None), -1, "no pages"), (dict(v_pages=None), -1, "no pages"),
-    (dict(k_pages=A + 8), -1, "16-byte aligned"), (dict(v_pages=A + 2), -1, "16-byte aligned"), (dict(mass=A + 2), -1, "4-byte aligned"),
+    (dict(k_pages=A + 8), -1, "16-byte aligned"), (dict(v_pages=A + 2), -1, "16-byte aligned"), (dict(mass=A + 4), -1, "16-byte aligned"),
+    (dict(pos=A + 8), -1, "16-byte aligned"),
 ])
 def test_refused_caches(mdx, call, over, rc, says):
     _refused(mdx, call, _cache(mdx, **over), _batch(mdx), rc, says)
