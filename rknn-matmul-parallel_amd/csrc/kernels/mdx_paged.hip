@@ -228,6 +228,9 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // masked place would be 0 * inf; outputs that are not finite therefore make the
 // wave run again with every tile checked, and tiles that hold such values take
 // the products of visible keys alone, in fp32.
+constexpr int kShort = 32;             // query rows up to which k_paged_attn takes a request
+constexpr int kRows = 128;             // query rows per block of k_paged_chunk
+
 struct AttnArgs {
     Paged p;
     const uint16_t* q;
@@ -236,9 +239,14 @@ struct AttnArgs {
     uint16_t* out;
     long long out_stride;
     float* lse;
-    float* part_o;             // [splits][n_tokens * nq][hd]
-    float2* part_ml;           // [splits][n_tokens * nq]: reference score, sum
-    int splits, split_keys;
+    // partial results of splits: unnormalised outputs; reference score and sum
+    float* short_o;            // k_paged_attn: [splits][n_req][nkv][short_rows][hd]
+    float2* short_ml;
+    int splits, split_keys, short_rows;
+    int short_max;             // the most query rows of a request that is k_paged_attn's
+    float* part_o;             // k_paged_chunk: [chunk_splits][n_tokens][nq][hd]
+    float2* part_ml;
+    int chunk_splits, chunk_keys;
 };
 
 // Probabilities are 2^(c (s - ref) + lift); the difference comes first, so that
@@ -275,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
     const int r = blockIdx.z, kvh = blockIdx.y % p.nkv, tile = blockIdx.y / p.nkv, split = blockIdx.x;
     const Req q = req_of(p, r);
     const int rows = min(q.n, p.max_q) * p.G;
-    if (tile * 16 >= rows) return;
+    if (tile * 16 >= rows || rows > a.short_max) return;
     const int R = min(tile * 16 + c16, rows - 1);    // this lane's query row (the last one repeated)
     const int tok = q.start + R / p.G, hq = kvh * p.G + R % p.G;
     const int vis = min(q.base + R / p.G + 1, p.limit);
@@ -433,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
         for (int j = 0; j < DJ; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) any = any + o[j][i] * 0.0f;
-        if (!__any(any != any)) break;
+        if (!__any(any != any && l == l)) break;     // (a sum that is none is one of scores)
     }
 
     l = rows_sum4(l);
@@ -475,11 +483,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
     }
     const int orow = tile * 16 + row, otok = q.start + orow / p.G, oh = kvh * p.G + orow % p.G;
     if (a.splits > 1) {
-        const size_t at = ((size_t)split * p.n_tokens + otok) * p.nq + oh;
-        float* po = a.part_o + at * HD + d0;
+        const size_t at = (((size_t)split * p.n_req + r) * p.nkv + kvh) * a.short_rows + orow;
+        float* po = a.short_o + at * HD + d0;
 #pragma unroll
         for (int j = 0; j < DJ; j += 4) *reinterpret_cast<float4*>(po + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        if (d0 == 0) a.part_ml[at] = make_float2(top, sum);
+        if (d0 == 0) a.short_ml[at] = make_float2(top, sum);
         return;
     }
     uint16_t* dst = a.out + (size_t)otok * a.out_stride + (size_t)oh * HD + d0;
@@ -489,41 +497,465 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
     if (a.lse && d0 == 0) a.lse[(size_t)otok * p.nq + oh] = row_lse<T>(top, sum, a.scale);
 }
 
-// Joins the splits of one row: a wave per row.
+// ---- attention: many query rows -----------------------------------------------------
+//
+// Requests with more than kShort query rows: a block takes 128 of them (new rows
+// x the group's heads) of one KV head against tiles of KB keys, 32 rows a wave, so
+// that a K or V fragment read from LDS feeds 32 rows.  Two groups of four waves
+// (one at 256 dimensions, for its registers) take alternate tiles and are joined
+// in LDS at the end: a CU holds one block, and two waves per SIMD let one's
+// exponentials run beside the other's products.
+//   S^T = K . Q^T    v_mfma_32x32x16: a lane holds half of its row's scores, the
+//                    lane 32 away the other half
+//   O^T = V^T . P^T  the scores' order in a lane is the k order of this product;
+//                    V^T comes out of row-major LDS by ds_read_b64_tr_b16
+// LDS rows have their 16-byte chunks permuted by the row number, so that neither
+// kind of read meets its own banks.  The accumulators of a score start at minus
+// the row's reference, which saves the subtraction in the exponent.
+// Probabilities go in rounded to the type once (the output's own rounding is as
+// large, and a second part would cost half as many products again); the sums are
+// of the unrounded ones.
+//
+// V rows that no row of the block sees are zeroed on their way to LDS.  Values
+// that are not finite at places that some rows see and others do not leave 0 * inf
+// behind: rows whose sum of weights is a number and whose output is not are
+// computed again by row_again, key by key in fp32.
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float16_t mfma32(_Float16, u32x4_t a, u32x4_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+}
+__device__ __forceinline__ float16_t mfma32(__bf16, u32x4_t a, u32x4_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0,
+                                                   0);
+}
+// Four rows of an LDS matrix, transposed: lane t of each 16 gives the address of
+// values 4 (t % 4) .. of row t / 4 and gets value t of the four rows.
+__device__ __forceinline__ uint2 lds_read_tr(const uint16_t* p) {
+    typedef __attribute__((address_space(3))) s16x4_t lds_t;
+    const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
+    return __builtin_bit_cast(uint2, v);
+}
+// The other 32 lanes' value.
+__device__ __forceinline__ float half_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// One query row over keys [k0, k1) by a wave, in fp32 and without matrix products:
+// the unnormalised outputs of dims (HD/64) lane .., their reference and sum.
 template <int HD, class T>
-__global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
+__device__ __noinline__ void row_again(const Paged& p, int r, int kvh, const uint16_t* qr, float c, int k0, int k1,
+                                       float* o, float* top, float* sum) {
     constexpr int DL = HD / 64;
-    const Paged& p = a.p;
     const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n_rows = (long long)p.n_tokens * p.nq;
-    if (row >= n_rows) return;
-    const int t = (int)(row / p.nq), h = (int)(row % p.nq);
-    const int r = find_req(p, t, lane);
-    if (r >= p.n_req) return;
+    float ref = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DL; d++) o[d] = 0.0f;
+    for (int kb = k0; kb < k1; kb += 64) {
+        const int j = kb + lane;
+        const long long at = j < k1 ? pool_row(p, r, kvh, j) : -1;
+        float s = -INFINITY;
+        if (at >= 0) {
+            s = 0.0f;
+            for (int d = 0; d < HD; d += 8) {
+                const u32x4_t k = *reinterpret_cast<const u32x4_t*>(p.kp + at * HD + d);
+                const u32x4_t q = *reinterpret_cast<const u32x4_t*>(qr + d);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    s = s + widen16<T>((uint16_t)k[w]) * widen16<T>((uint16_t)q[w]);
+                    s = s + widen16<T>((uint16_t)(k[w] >> 16)) * widen16<T>((uint16_t)(q[w] >> 16));
+                }
+            }
+        }
+        const float mx = fmaxf(wave_max(s), ref);
+        if (mx == -INFINITY) continue;
+        const float alpha = ref_weight(ref, mx, c);
+        const float w = at >= 0 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s - mx, c, kLift<T>)) : 0.0f;
+        ref = mx;
+        l = l * alpha + wave_sum(w);
+#pragma unroll
+        for (int d = 0; d < DL; d++) o[d] = o[d] * alpha;
+        for (int i = 0; i < 64; i++) {
+            const long long v = __shfl(at, i, kWave);
+            if (v < 0) continue;
+            const float wi = __shfl(w, i, kWave);
+#pragma unroll
+            for (int d = 0; d < DL; d++) o[d] = o[d] + wi * widen16<T>(p.vp[v * HD + DL * lane + d]);
+        }
+    }
+    *top = ref;
+    *sum = l;
+}
+
+template <int HD, class T>
+__global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_paged_chunk(AttnArgs a) {
+    constexpr int GR = HD == 256 ? 1 : 2;           // groups of four waves
+    constexpr int KB = HD == 256 ? 32 : 64;         // keys per tile
+    constexpr int CH = HD / 8;                      // 16-byte chunks per row
+    constexpr int SW = CH < 16 ? CH - 1 : 15;       // rows whose chunks are permuted apart
+    constexpr int DS = HD / 16, DT = HD / 32, KT = KB / 32;
+    constexpr int U = KB * CH / 256;                // chunks per thread and tile
+    constexpr int RPU = 256 / CH;                   // rows per round of chunks
+    constexpr int TN = KB * HD;                     // values per tile
+    __shared__ __attribute__((aligned(16))) uint16_t lds[GR * 2 * 2 * TN];
+    __shared__ int again;
+
+    const Paged& p = a.p;
+    const int grp = GR == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int hi = lane >> 5, c32 = lane & 31;
+    const int kvh = blockIdx.x % p.nkv;
+
+    // the request and the block of rows in it: the last ones (the longest) first
+    int r = -1, tile = 0;
+    {
+        int total = 0;
+        for (int pass = 0; pass < 2 && r < 0; pass++) {
+            const int want = total - 1 - (int)(blockIdx.x / p.nkv);
+            if (pass == 1 && want < 0) return;
+            int before = 0;
+            for (int j0 = 0; j0 < p.n_req; j0 += 64) {
+                int t = 0;
+                if (j0 + lane < p.n_req) {
+                    const Req q = req_of(p, j0 + lane);
+                    const int rows = min(q.n, p.max_q) * p.G;
+                    t = rows > a.short_max ? (rows + kRows - 1) / kRows : 0;
+                }
+                int incl = t;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int y = __shfl_up(incl, o, kWave);
+                    if (lane >= o) incl += y;
+                }
+                if (pass == 1) {
+                    const unsigned long long hit = __ballot(before + incl > want);
+                    if (hit) {
+                        const int src = __builtin_ctzll(hit);
+                        r = j0 + src;
+                        tile = want - (before + __shfl(incl - t, src, kWave));
+                        break;
+                    }
+                }
+                before += __shfl(incl, 63, kWave);
+            }
+            total = before;
+        }
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
+    tile = __builtin_amdgcn_readfirstlane(tile);
     const Req q = req_of(p, r);
-    const int i = t - q.start, n = min(q.n, p.max_q);
-    if (i < 0 || i >= n) return;
-    const int tile = (i * p.G + h % p.G) / 16;
-    const int kend = min(q.base + min(tile * 16 + 15, n * p.G - 1) / p.G + 1, p.limit);
-    const int ns = max((kend + a.split_keys - 1) / a.split_keys, 1);
+    const int rows = min(q.n, p.max_q) * p.G, row0 = tile * kRows;
+    const int R = min(row0 + 32 * wave + c32, rows - 1);
+    const int tok = q.start + R / p.G, hq = kvh * p.G + R % p.G;
+    const int vis = min(q.base + R / p.G + 1, p.limit);
+    const int vmin = min(q.base + row0 / p.G + 1, p.limit);
+    const int kend = min(q.base + min(row0 + kRows - 1, rows - 1) / p.G + 1, p.limit);
+    const int split = blockIdx.y;
+    const int k0 = split * a.chunk_keys, k1 = min(kend, k0 + a.chunk_keys);
+    if (k0 >= k1 && split > 0) return;
+
+    u32x4_t qf[DS];
+    {
+        const uint16_t* qr = a.q + (size_t)tok * a.q_stride + (size_t)hq * HD + 8 * hi;
+#pragma unroll
+        for (int s = 0; s < DS; s++) qf[s] = *reinterpret_cast<const u32x4_t*>(qr + 16 * s);
+    }
+
+    // staging: round i of this thread is chunk tid % CH of row tid / CH + i RPU; a
+    // wave's rows of a round lie in 16 keys, so in one page
+    const int* table = p.table + (size_t)r * p.max_pages;
+    const int pmask = (1 << p.shift) - 1;
+    const int srow = tid / CH, sch = tid % CH, wrow = wave * (64 / CH);
+    u32x4_t kr[U], vr[U];
+    auto load = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int key = kb + ((wrow + i * RPU) & ~15);
+            const int pg = key < k1 ? table[key >> p.shift] : -1;
+            const bool ok = (unsigned)pg < (unsigned)p.n_pages;
+            const size_t at = ((((size_t)(ok ? pg : 0) * p.nkv + kvh) << p.shift) + (key & pmask) + ((srow + i * RPU) & 15)) * HD + 8 * sch;
+            kr[i] = *reinterpret_cast<const u32x4_t*>(p.kp + at);
+            vr[i] = *reinterpret_cast<const u32x4_t*>(p.vp + at);
+            if (!ok || kb + srow + i * RPU >= kend) vr[i] = u32x4_t{0u, 0u, 0u, 0u};
+        }
+    };
+    uint16_t* const kbuf = lds + grp * 4 * TN;      // [2][K tile, V tile]
+    auto stash = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int row = srow + i * RPU, at = row * HD + 8 * (sch ^ (row & SW));
+            *reinterpret_cast<u32x4_t*>(kbuf + buf * 2 * TN + at) = kr[i];
+            *reinterpret_cast<u32x4_t*>(kbuf + buf * 2 * TN + TN + at) = vr[i];
+        }
+    };
+
+    float16_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float ref = -INFINITY, l = 0.0f;
+    bool seen = false;
+
+    const int nt = (k1 - k0 + KB - 1) / KB;
+    load(k0 + grp * KB);
+    stash(0);
+    load(k0 + (grp + GR) * KB);
+    if (threadIdx.x == 0) again = 0;
+    __syncthreads();
+    for (int t0 = 0; t0 < nt; t0 += GR) {
+        const int t = t0 + grp, kb = k0 + t * KB, buf = (t0 / GR) & 1;
+        stash(buf ^ 1);
+        load(kb + 2 * GR * KB);
+        const uint16_t* ks = kbuf + buf * 2 * TN;
+        const uint16_t* vs = ks + TN;
+        if (t < nt) {
+            const float start = ref == -INFINITY ? 0.0f : -ref;
+            float16_t s[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[kt][i] = start;
+#pragma unroll
+                for (int d = 0; d < DS; d++) {
+                    const int row = 32 * kt + c32;
+                    const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(ks + row * HD + 8 * ((2 * d + hi) ^ (row & SW)));
+                    s[kt] = mfma32(T(), kf, qf[d], s[kt]);
+                }
+            }
+            // pages that do not exist, and keys that some row does not see
+            int okbits = 0;
+#pragma unroll
+            for (int u = 0; u < KB / 16; u++) {
+                const int key = kb + 16 * u;
+                const int pg = key < k1 ? table[key >> p.shift] : -1;
+                if ((unsigned)pg < (unsigned)p.n_pages) okbits |= 1 << u;
+            }
+            if (kb + KB > vmin || okbits != (1 << (KB / 16)) - 1) {
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int key = 32 * kt + 8 * (i >> 2) + (i & 3);     // + 4 hi
+                        if (!((okbits >> (key >> 4)) & 1) || kb + key + 4 * hi >= vis) s[kt][i] = -INFINITY;
+                        else seen = true;
+                    }
+            } else {
+                seen = true;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kt][i]);
+            mx = half_max(mx);
+            const bool move = ref == -INFINITY ? mx > -INFINITY : mx * a.c > 8.0f;
+            if (__any(move)) {
+                const float delta = move ? mx : 0.0f;
+                const float alpha = !move ? 1.0f : (ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-delta * a.c));
+                if (move) ref = delta - start;
+                l = l * alpha;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * alpha;
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[kt][i] = s[kt][i] - delta;
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    s[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.c, kLift<T>));
+                    l = l + s[kt][i];
+                }
+#pragma unroll
+            for (int kk = 0; kk < KB / 16; kk++) {
+                u32x4_t pf;
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    pf[w] = pack16<T>(s[kk >> 1][8 * (kk & 1) + 2 * w], s[kk >> 1][8 * (kk & 1) + 2 * w + 1]);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const int key = 16 * kk + 4 * hi + ((lane & 15) >> 2);
+                    const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                    const uint2 v0 = lds_read_tr(vs + key * HD + 8 * ((col >> 3) ^ (key & SW)) + (col & 7));
+                    const uint2 v1 = lds_read_tr(vs + (key + 8) * HD + 8 * ((col >> 3) ^ ((key + 8) & SW)) + (col & 7));
+                    o[d] = mfma32(T(), u32x4_t{v0.x, v0.y, v1.x, v1.y}, pf, o[d]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    // group 1's sums, brought to a common reference
+    l = half_sum(l);
+    if (ref == -INFINITY && l == l) l = seen ? 1.0f : 0.0f;
+    float* const mg = reinterpret_cast<float*>(lds);
+    static_assert(GR == 1 || (16 * DT + 2) * 256 * 4 <= (int)sizeof lds, "the merge fits the tiles");
+    if (GR == 2) {
+        if (grp == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mg[(16 * d + i) * 256 + tid] = o[d][i];
+            mg[16 * DT * 256 + tid] = ref;
+            mg[(16 * DT + 1) * 256 + tid] = l;
+        }
+        __syncthreads();
+    }
+    const bool rv = row0 + 32 * wave + c32 < rows;
+    bool redo = false;
+    if (grp == 0) {
+        if (GR == 2) {
+            const float ref1 = mg[16 * DT * 256 + tid], l1 = mg[(16 * DT + 1) * 256 + tid], top = fmaxf(ref, ref1);
+            const float w0 = ref_weight(ref, top, a.c), w1 = ref_weight(ref1, top, a.c);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * w0 + mg[(16 * d + i) * 256 + tid] * w1;
+            l = l * w0 + l1 * w1;
+            ref = top;
+        }
+        float any = 0.0f;                  // NaN when an output is not finite
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) any = any + o[d][i] * 0.0f;
+        redo = rv && any != any && l == l;
+        if (redo) again = 1;
+        const size_t row = (size_t)tok * p.nq + hq;
+        if (rv && a.chunk_splits > 1) {
+            float* po = a.part_o + ((size_t)split * p.n_tokens * p.nq + row) * HD + 4 * hi;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4*>(po + 32 * d + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+            if (hi == 0) a.part_ml[(size_t)split * p.n_tokens * p.nq + row] = make_float2(ref, l);
+        } else if (rv) {
+            uint16_t* dst = a.out + (size_t)tok * a.out_stride + (size_t)hq * HD + 4 * hi;
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = ref == -INFINITY ? row_result(0.0f, ref, l) : o[d][i + e] * inv;
+                    *reinterpret_cast<uint2*>(dst + 32 * d + 2 * i) = make_uint2(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]));
+                }
+            if (a.lse && hi == 0) a.lse[row] = row_lse<T>(ref, l, a.scale);
+        }
+    }
+    __syncthreads();
+    if (!again || grp != 0) return;
+    unsigned long long todo = __ballot(redo);
+    todo = (todo | (todo >> 32)) & 0xffffffffull;
+    while (todo) {
+        const int c = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int R2 = row0 + 32 * wave + c, t2 = q.start + R2 / p.G, h2 = kvh * p.G + R2 % p.G;
+        float x[HD / 64], top, sum;
+        row_again<HD, T>(p, r, kvh, a.q + (size_t)t2 * a.q_stride + (size_t)h2 * HD, a.c, k0,
+                         min(k1, min(q.base + R2 / p.G + 1, p.limit)), x, &top, &sum);
+        const size_t row = (size_t)t2 * p.nq + h2;
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) {
+            const int at = HD / 64 * lane + d;
+            if (a.chunk_splits > 1) a.part_o[((size_t)split * p.n_tokens * p.nq + row) * HD + at] = x[d];
+            else a.out[(size_t)t2 * a.out_stride + (size_t)h2 * HD + at] = bits16<T>(row_result(x[d], top, sum));
+        }
+        if (a.chunk_splits > 1 && lane == 0) a.part_ml[(size_t)split * p.n_tokens * p.nq + row] = make_float2(top, sum);
+    }
+}
+
+// Joins the splits of a row: W waves per row.  Rows of a short request lie at
+// ((split * n_req + r) * nkv + KV head) * short_rows + row of the short partials,
+// the others at split * n_tokens * nq + token * nq + head.
+template <int HD, class T, int W>
+__global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
+    constexpr int DL = HD / 64, RB = 4 / W;
+    __shared__ float osh[4][HD + 4];
+    const Paged& p = a.p;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % W;
+    const float* part_o;
+    const float2* part_ml;
+    size_t step;
+    int t, h, kend, keys;
+    if (W == 4) {
+        // a block per short row
+        const int r = blockIdx.z, kvh = blockIdx.y, R = blockIdx.x;
+        const Req q = req_of(p, r);
+        const int rows = min(q.n, p.max_q) * p.G;
+        if (R >= rows || rows > a.short_max) return;
+        const int tile = R / 16;
+        t = q.start + R / p.G;
+        h = kvh * p.G + R % p.G;
+        kend = min(q.base + min(tile * 16 + 15, rows - 1) / p.G + 1, p.limit);
+        keys = a.split_keys;
+        step = (size_t)p.n_req * p.nkv * a.short_rows;
+        const size_t row = ((size_t)r * p.nkv + kvh) * a.short_rows + R;
+        part_o = a.short_o + row * HD;
+        part_ml = a.short_ml + row;
+    } else {
+        const long long row = (long long)blockIdx.x * RB + wave / W;
+        if (row >= (long long)p.n_tokens * p.nq) return;
+        t = (int)(row / p.nq);
+        h = (int)(row % p.nq);
+        const int r = find_req(p, t, lane);
+        if (r >= p.n_req) return;
+        const Req q = req_of(p, r);
+        const int i = t - q.start, rows = min(q.n, p.max_q) * p.G, R = i * p.G + h % p.G;
+        if (i < 0 || R >= rows || rows <= a.short_max) return;
+        kend = min(q.base + min(R / kRows * kRows + kRows - 1, rows - 1) / p.G + 1, p.limit);
+        keys = a.chunk_keys;
+        step = (size_t)p.n_tokens * p.nq;
+        part_o = a.part_o + row * HD;
+        part_ml = a.part_ml + row;
+    }
+    const int ns = max((kend + keys - 1) / keys, 1);
     float top = -INFINITY;
-    for (int s = lane; s < ns; s += 64) top = fmaxf(top, a.part_ml[s * n_rows + row].x);
+    for (int s = lane; s < ns; s += 64) top = fmaxf(top, part_ml[s * step].x);
     top = wave_max(top);
     float sum = 0.0f, v[DL];
 #pragma unroll
     for (int d = 0; d < DL; d++) v[d] = 0.0f;
-    for (int s = 0; s < ns; s++) {
-        const float2 ml = a.part_ml[s * n_rows + row];
+#pragma unroll 4
+    for (int s = sub; s < ns; s += W) {
+        const float2 ml = part_ml[s * step];
         const float w = ref_weight(ml.x, top, a.c);
         sum = sum + ml.y * w;
-        const float* po = a.part_o + (s * n_rows + row) * HD + DL * lane;
+        const float* po = part_o + s * step * HD + DL * lane;
 #pragma unroll
         for (int d = 0; d < DL; d++) v[d] = v[d] + po[d] * w;
+    }
+    if (W > 1) {
+#pragma unroll
+        for (int d = 0; d < DL; d++) osh[wave][DL * lane + d] = v[d];
+        if (lane == 0) osh[wave][HD] = sum;
+        __syncthreads();
+        if (sub != 0) return;
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+#pragma unroll
+            for (int d = 0; d < DL; d++) v[d] = v[d] + osh[w][DL * lane + d];
+            sum = sum + osh[w][HD];
+        }
     }
     uint16_t* dst = a.out + (size_t)t * a.out_stride + (size_t)h * HD + DL * lane;
 #pragma unroll
     for (int d = 0; d < DL; d++) dst[d] = bits16<T>(row_result(v[d], top, sum));
-    if (a.lse && lane == 0) a.lse[row] = row_lse<T>(top, sum, a.scale);
+    if (a.lse && lane == 0) a.lse[(size_t)t * p.nq + h] = row_lse<T>(top, sum, a.scale);
 }
 
 // ---- received weight ---------------------------------------------------------------
@@ -815,22 +1247,49 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
 
 // ---- shapes -----------------------------------------------------------------------------
 
-struct Splits {
-    int n, keys;
+// How a batch is cut up.  Short requests: enough workgroups for the chip, but
+// splits of at least 256 keys; the others: splits only while there are fewer
+// blocks than CUs.
+struct Plan {
+    int short_max;
+    int tiles, splits, split_keys, short_rows;           // k_paged_attn (tiles 0: not launched)
+    int blocks, chunk_splits, chunk_keys;                // k_paged_chunk (blocks 0: not launched)
 };
-// Enough workgroups for the chip, but splits of at least 256 keys.
-Splits attn_splits(const Paged& p) {
-    const long long blocks = (long long)p.n_req * p.nkv * cdiv((long long)p.max_q * p.G, 16);
-    long long want = cdiv(1024, blocks > 0 ? blocks : 1);
-    const long long most = cdiv(p.limit > 0 ? p.limit : 1, 256);
-    if (want > most) want = most;
-    Splits s;
-    s.keys = cdiv(cdiv(p.limit > 0 ? p.limit : 1, want), 128) * 128;
-    s.n = cdiv(p.limit > 0 ? p.limit : 1, s.keys);
+Plan attn_plan(const Paged& p) {
+    Plan s = {};
+    const int limit = p.limit > 0 ? p.limit : 1;
+    const long long rows = (long long)p.max_q * p.G;
+    s.short_rows = rows < kShort ? (int)rows : kShort;
+    // with as many rows as all requests can have, none is expected to be short (one
+    // that is all the same is taken along by k_paged_chunk)
+    s.short_max = rows > kShort && (long long)p.n_req * p.max_q <= p.n_tokens ? 0 : kShort;
+    if (s.short_max) {
+        s.tiles = cdiv(s.short_rows, 16);
+        long long want = cdiv(1024, (long long)p.n_req * p.nkv * s.tiles);
+        const long long most = cdiv(limit, 256);
+        if (want > most) want = most;
+        s.split_keys = cdiv(cdiv(limit, want), 128) * 128;
+        s.splits = cdiv(limit, s.split_keys);
+    }
+    if (rows > kShort) {
+        long long n = (long long)p.n_tokens * p.G / kRows + p.n_req;
+        const long long each = (long long)p.n_req * cdiv(rows, kRows);
+        if (n > each) n = each;
+        s.blocks = (int)n;
+        long long want = 256 / (n * p.nkv);
+        const long long most = cdiv(limit, 512);
+        want = want < 1 ? 1 : (want > most ? most : want);
+        s.chunk_keys = cdiv(cdiv(limit, want), 128) * 128;
+        s.chunk_splits = cdiv(limit, s.chunk_keys);
+    }
     return s;
 }
-
-size_t attn_rows(const Paged& p) { return (size_t)p.n_tokens * p.nq; }
+size_t short_parts(const Paged& p, const Plan& s) {
+    return s.tiles && s.splits > 1 ? (size_t)s.splits * p.n_req * p.nkv * s.short_rows : 0;
+}
+size_t chunk_parts(const Paged& p, const Plan& s) {
+    return s.blocks && s.chunk_splits > 1 ? (size_t)s.chunk_splits * p.n_tokens * p.nq : 0;
+}
 
 }  // namespace
 
@@ -849,10 +1308,16 @@ void append_launch(const AppendArgs& a, hipStream_t s) {
 }
 
 template <int HD, class T>
-void attn_launch(const AttnArgs& a, int tiles, hipStream_t s) {
-    hipLaunchKernelGGL((k_paged_attn<HD, T>), dim3(a.splits, a.p.nkv * tiles, a.p.n_req), dim3(256), 0, s, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL((k_paged_join<HD, T>), dim3(cdiv((long long)attn_rows(a.p), 4)), dim3(256), 0, s, a);
+void attn_launch(const AttnArgs& a, const Plan& s, hipStream_t st) {
+    if (s.blocks)
+        hipLaunchKernelGGL((k_paged_chunk<HD, T>), dim3(s.blocks * a.p.nkv, s.chunk_splits), dim3(HD == 256 ? 256 : 512),
+                           0, st, a);
+    if (s.tiles)
+        hipLaunchKernelGGL((k_paged_attn<HD, T>), dim3(s.splits, a.p.nkv * s.tiles, a.p.n_req), dim3(256), 0, st, a);
+    if (chunk_parts(a.p, s))
+        hipLaunchKernelGGL((k_paged_join<HD, T, 1>), dim3(cdiv((long long)a.p.n_tokens * a.p.nq, 4)), dim3(256), 0, st, a);
+    if (short_parts(a.p, s))
+        hipLaunchKernelGGL((k_paged_join<HD, T, 4>), dim3(s.short_rows, a.p.nkv, a.p.n_req), dim3(256), 0, st, a);
 }
 
 template <int HD, class T>
@@ -888,8 +1353,9 @@ int mdx_launch_paged_append(const MdxPagedCache* c, const MdxPagedBatch* b, cons
 
 size_t mdx_paged_attn_scratch(const MdxPagedCache* c, const MdxPagedBatch* b) {
     const Paged p = paged(c, b);
-    const Splits s = attn_splits(p);
-    return s.n > 1 ? (size_t)s.n * attn_rows(p) * ((size_t)c->head_dim * 4 + 8) : 0;
+    if (p.max_q == 0) return 0;
+    const Plan s = attn_plan(p);
+    return (short_parts(p, s) + chunk_parts(p, s)) * ((size_t)c->head_dim * 4 + 8);
 }
 
 int mdx_launch_paged_attn(const MdxPagedCache* c, const MdxPagedBatch* b, const void* q, long long q_stride,
@@ -897,7 +1363,7 @@ int mdx_launch_paged_attn(const MdxPagedCache* c, const MdxPagedBatch* b, const 
     AttnArgs a = {};
     a.p = paged(c, b);
     if (a.p.max_q == 0) return 0;
-    const Splits s = attn_splits(a.p);
+    const Plan s = attn_plan(a.p);
     a.q = (const uint16_t*)q;
     a.q_stride = q_stride;
     a.scale = scale;
@@ -905,13 +1371,19 @@ int mdx_launch_paged_attn(const MdxPagedCache* c, const MdxPagedBatch* b, const 
     a.out = (uint16_t*)out;
     a.out_stride = out_stride;
     a.lse = lse;
-    a.splits = s.n;
-    a.split_keys = s.keys;
-    a.part_o = (float*)scratch;
-    a.part_ml = (float2*)((float*)scratch + (s.n > 1 ? (size_t)s.n * attn_rows(a.p) * c->head_dim : 0));
-    const long long tiles = cdiv((long long)a.p.max_q * a.p.G, 16);
-    if (tiles * a.p.nkv > 65535) return mdxrt_refuse(-1, "mdx_paged_attention: max_q_len is too large");
-    MDX_PAGED_HD(attn_launch, a, (int)tiles, (hipStream_t)stream);
+    const size_t ns = short_parts(a.p, s), nc = chunk_parts(a.p, s), hd = c->head_dim;
+    a.splits = s.splits;
+    a.split_keys = s.split_keys;
+    a.short_rows = s.short_rows;
+    a.short_max = s.short_max;
+    a.chunk_splits = s.chunk_splits;
+    a.chunk_keys = s.chunk_keys;
+    a.short_o = (float*)scratch;
+    a.part_o = a.short_o + ns * hd;
+    a.short_ml = (float2*)(a.part_o + nc * hd);
+    a.part_ml = a.short_ml + ns;
+    if ((long long)s.blocks * a.p.nkv > 0x7fffffffLL) return mdxrt_refuse(-1, "mdx_paged_attention: too many rows");
+    MDX_PAGED_HD(attn_launch, a, s, (hipStream_t)stream);
     return mdxrt_launched("mdx_paged_attention");
 }
 
