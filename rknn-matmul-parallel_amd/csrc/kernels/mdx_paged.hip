@@ -102,7 +102,9 @@ __device__ __forceinline__ float widen16(uint16_t b) {
 }
 template <class T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
-    return (uint32_t)bits16<T>(a) | ((uint32_t)bits16<T>(b) << 16);
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    typedef T t2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{a, b}), t2_t));
 }
 
 __device__ __forceinline__ float4_t mfma16(_Float16, u32x4_t a, u32x4_t b, float4_t c) {
@@ -510,8 +512,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
 //   O^T = V^T . P^T  the scores' order in a lane is the k order of this product;
 //                    V^T comes out of row-major LDS by ds_read_b64_tr_b16
 // LDS rows have their 16-byte chunks permuted by the row number, so that neither
-// kind of read meets its own banks.  The accumulators of a score start at minus
-// the row's reference, which saves the subtraction in the exponent.
+// kind of read meets its own banks.
 // Probabilities go in rounded to the type once (the output's own rounding is as
 // large, and a second part would cost half as many products again); the sums are
 // of the unrounded ones.
@@ -551,7 +552,7 @@ __device__ __forceinline__ float half_sum(float v) {
 // One query row over keys [k0, k1) by a wave, in fp32 and without matrix products:
 // the unnormalised outputs of dims (HD/64) lane .., their reference and sum.
 template <int HD, class T>
-__device__ __noinline__ void row_again(const Paged& p, int r, int kvh, const uint16_t* qr, float c, int k0, int k1,
+__device__ __forceinline__ void row_again(const Paged& p, int r, int kvh, const uint16_t* qr, float c, int k0, int k1,
                                        float* o, float* top, float* sum) {
     constexpr int DL = HD / 64;
     const int lane = threadIdx.x & 63;
@@ -668,26 +669,52 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         for (int s = 0; s < DS; s++) qf[s] = *reinterpret_cast<const u32x4_t*>(qr + 16 * s);
     }
 
-    // staging: round i of this thread is chunk tid % CH of row tid / CH + i RPU; a
-    // wave's rows of a round lie in 16 keys, so in one page
+    // Staging: round i of this thread is chunk tid % CH of row tid / CH + i RPU; a
+    // wave's rows of a round lie in 16 keys, so in one page.  A tile's page numbers
+    // are read two tiles before its rows are requested, and these one tile before
+    // they go to LDS, so that nothing waits for what it has just asked for.
     const int* table = p.table + (size_t)r * p.max_pages;
     const int pmask = (1 << p.shift) - 1;
-    const int srow = tid / CH, sch = tid % CH, wrow = wave * (64 / CH);
+    const int srow = tid / CH, sch = tid % CH;
+    constexpr int NG = KB / 16;                     // 16-key groups of a tile
+    int pg[NG];
+    auto pages = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NG; u++) pg[u] = table[min(kb + 16 * u, k1 - 1) >> p.shift];
+    };
+    // (wrow + i RPU) / 16
+    auto group = [&](int i) __attribute__((always_inline)) -> int {
+        return CH == 8 ? 2 * i + (wave >> 1) : (CH == 16 ? i : i >> 1);
+    };
     u32x4_t kr[U], vr[U];
-    auto load = [&](int kb) __attribute__((always_inline)) {
+    const size_t head = (size_t)kvh << p.shift;
+    // requests the tile whose page numbers are in pg; returns which of them exist
+    auto load = [&](int kb) __attribute__((always_inline)) -> int {
+        int bits = 0;
+#pragma unroll
+        for (int u = 0; u < NG; u++) {
+            const bool ok = kb + 16 * u < k1 && (unsigned)pg[u] < (unsigned)p.n_pages;
+            bits |= ok ? 1 << u : 0;
+            pg[u] = ok ? pg[u] : 0;
+        }
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const int key = kb + ((wrow + i * RPU) & ~15);
-            const int pg = key < k1 ? table[key >> p.shift] : -1;
-            const bool ok = (unsigned)pg < (unsigned)p.n_pages;
-            const size_t at = ((((size_t)(ok ? pg : 0) * p.nkv + kvh) << p.shift) + (key & pmask) + ((srow + i * RPU) & 15)) * HD + 8 * sch;
-            kr[i] = *reinterpret_cast<const u32x4_t*>(p.kp + at);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(p.vp + at);
-            if (!ok || kb + srow + i * RPU >= kend) vr[i] = u32x4_t{0u, 0u, 0u, 0u};
+            const int u = group(i);
+            const int page = CH == 8 ? ((wave >> 1) ? pg[2 * i + 1] : pg[2 * i]) : pg[CH == 16 ? i : i >> 1];
+            const size_t base = ((((size_t)page * p.nkv) << p.shift) + head + ((kb + 16 * u) & pmask)) * HD;
+            const unsigned at = ((srow + i * RPU) & 15) * HD + 8 * sch;
+            kr[i] = *reinterpret_cast<const u32x4_t*>(p.kp + base + at);
+            vr[i] = *reinterpret_cast<const u32x4_t*>(p.vp + base + at);
         }
+        return bits;
     };
     uint16_t* const kbuf = lds + grp * 4 * TN;      // [2][K tile, V tile]
-    auto stash = [&](int buf) __attribute__((always_inline)) {
+    auto stash = [&](int buf, int kb, int bits) __attribute__((always_inline)) {
+        if (kb + KB > kend || bits != (1 << NG) - 1) {
+#pragma unroll
+            for (int i = 0; i < U; i++)
+                if (!((bits >> group(i)) & 1) || kb + srow + i * RPU >= kend) vr[i] = u32x4_t{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (int i = 0; i < U; i++) {
             const int row = srow + i * RPU, at = row * HD + 8 * (sch ^ (row & SW));
@@ -695,6 +722,18 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
             *reinterpret_cast<u32x4_t*>(kbuf + buf * 2 * TN + TN + at) = vr[i];
         }
     };
+    // where this lane reads: K rows c32 (+ 32 kt), chunk 2 d + hi; V rows 4 hi + ..
+    // (+ 16 kk, + 8), four values of column 32 d + ..
+    int kat[DS], vat[DT][2];
+#pragma unroll
+    for (int d = 0; d < DS; d++) kat[d] = grp * 4 * TN + c32 * HD + 8 * ((2 * d + hi) ^ (c32 & SW));
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int key = 8 * e + 4 * hi + ((lane & 15) >> 2), col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            vat[d][e] = grp * 4 * TN + TN + key * HD + 8 * ((col >> 3) ^ (key & SW)) + (col & 7);
+        }
 
     float16_t o[DT];
 #pragma unroll
@@ -704,97 +743,133 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     float ref = -INFINITY, l = 0.0f;
     bool seen = false;
 
-    const int nt = (k1 - k0 + KB - 1) / KB;
-    load(k0 + grp * KB);
-    stash(0);
-    load(k0 + (grp + GR) * KB);
-    if (threadIdx.x == 0) again = 0;
-    __syncthreads();
-    for (int t0 = 0; t0 < nt; t0 += GR) {
-        const int t = t0 + grp, kb = k0 + t * KB, buf = (t0 / GR) & 1;
-        stash(buf ^ 1);
-        load(kb + 2 * GR * KB);
-        const uint16_t* ks = kbuf + buf * 2 * TN;
-        const uint16_t* vs = ks + TN;
-        if (t < nt) {
-            const float start = ref == -INFINITY ? 0.0f : -ref;
-            float16_t s[KT];
+    auto tile_step = [&](int buf, int kb, int bits) __attribute__((always_inline)) {
+        const uint16_t* ks = lds + buf * 2 * TN;
+        float16_t s[KT];
+        u32x4_t kf[2][DS];
 #pragma unroll
-            for (int kt = 0; kt < KT; kt++) {
+        for (int d = 0; d < DS; d++) kf[0][d] = *reinterpret_cast<const u32x4_t*>(ks + kat[d]);
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[kt][i] = start;
+        for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
-                for (int d = 0; d < DS; d++) {
-                    const int row = 32 * kt + c32;
-                    const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(ks + row * HD + 8 * ((2 * d + hi) ^ (row & SW)));
-                    s[kt] = mfma32(T(), kf, qf[d], s[kt]);
-                }
+            for (int i = 0; i < 16; i++) s[kt][i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DS; d++) {
+                s[kt] = mfma32(T(), kf[kt & 1][d], qf[d], s[kt]);
+                if (kt + 1 < KT) kf[(kt + 1) & 1][d] = *reinterpret_cast<const u32x4_t*>(ks + kat[d] + 32 * (kt + 1) * HD);
             }
+        }
+        uint2 vf[2][DT][2];
+        auto vload = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) vf[kk & 1][d][e] = lds_read_tr(ks + vat[d][e] + 16 * kk * HD);
+        };
+        vload(0);
+        // fragments ahead of the products that take them
+        __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+#pragma unroll
+        for (int i = 0; i < DS * (KT - 1); i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
+        if (kb + KB > vmin || bits != (1 << NG) - 1) {
             // pages that do not exist, and keys that some row does not see
-            int okbits = 0;
-#pragma unroll
-            for (int u = 0; u < KB / 16; u++) {
-                const int key = kb + 16 * u;
-                const int pg = key < k1 ? table[key >> p.shift] : -1;
-                if ((unsigned)pg < (unsigned)p.n_pages) okbits |= 1 << u;
-            }
-            if (kb + KB > vmin || okbits != (1 << (KB / 16)) - 1) {
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = 32 * kt + 8 * (i >> 2) + (i & 3);     // + 4 hi
-                        if (!((okbits >> (key >> 4)) & 1) || kb + key + 4 * hi >= vis) s[kt][i] = -INFINITY;
-                        else seen = true;
-                    }
-            } else {
-                seen = true;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kt][i]);
-            mx = half_max(mx);
-            const bool move = ref == -INFINITY ? mx > -INFINITY : mx * a.c > 8.0f;
-            if (__any(move)) {
-                const float delta = move ? mx : 0.0f;
-                const float alpha = !move ? 1.0f : (ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-delta * a.c));
-                if (move) ref = delta - start;
-                l = l * alpha;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * alpha;
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) s[kt][i] = s[kt][i] - delta;
-            }
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    s[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.c, kLift<T>));
-                    l = l + s[kt][i];
+                    const int key = 32 * kt + 8 * (i >> 2) + (i & 3);     // + 4 hi
+                    if (!((bits >> (key >> 4)) & 1) || kb + key + 4 * hi >= vis) s[kt][i] = -INFINITY;
+                    else seen = true;
                 }
+        } else {
+            seen = true;
+        }
+        float m4[4];
 #pragma unroll
-            for (int kk = 0; kk < KB / 16; kk++) {
-                u32x4_t pf;
+        for (int e = 0; e < 4; e++) {
+            m4[e] = s[0][e];
 #pragma unroll
-                for (int w = 0; w < 4; w++)
-                    pf[w] = pack16<T>(s[kk >> 1][8 * (kk & 1) + 2 * w], s[kk >> 1][8 * (kk & 1) + 2 * w + 1]);
+            for (int i = 4 + e; i < 16 * KT; i += 4) m4[e] = fmaxf(m4[e], s[i >> 4][i & 15]);
+        }
+        const float mx = half_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        const float next = (mx - ref) * a.c > 8.0f ? mx : ref;
+        if (__any(next != ref)) {
+            const float alpha = ref_weight(ref, next, a.c);
+            l = l * alpha;
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const int key = 16 * kk + 4 * hi + ((lane & 15) >> 2);
-                    const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                    const uint2 v0 = lds_read_tr(vs + key * HD + 8 * ((col >> 3) ^ (key & SW)) + (col & 7));
-                    const uint2 v1 = lds_read_tr(vs + (key + 8) * HD + 8 * ((col >> 3) ^ ((key + 8) & SW)) + (col & 7));
-                    o[d] = mfma32(T(), u32x4_t{v0.x, v0.y, v1.x, v1.y}, pf, o[d]);
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * alpha;
+            ref = next;
+        }
+        // the reference's exponent, rounded, is one factor of all probabilities
+        // of the row; where a step of it is no longer small, the scores are taken
+        // relative to the reference first
+        float off = ref == -INFINITY ? 0.0f : __builtin_fmaf(-ref, a.c, kLift<T>);
+        if (__any(fabsf(off) > 0x1p20f)) {
+            const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[kt][i] = s[kt][i] - base;
+            off = kLift<T>;
+        }
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; kk++) {
+            u32x4_t pf;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][8 * (kk & 1) + 2 * w + e], a.c, off));
+                    l4[2 * (w & 1) + e] = l4[2 * (w & 1) + e] + x[e];
                 }
+                pf[w] = pack16<T>(x[0], x[1]);
+            }
+            if (kk + 1 < KB / 16) vload(kk + 1);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const uint2 v0 = vf[kk & 1][d][0], v1 = vf[kk & 1][d][1];
+                o[d] = mfma32(T(), u32x4_t{v0.x, v0.y, v1.x, v1.y}, pf, o[d]);
             }
         }
+        l = l + ((l4[0] + l4[1]) + (l4[2] + l4[3]));
+    };
+
+    const int nt = (k1 - k0 + KB - 1) / KB;
+    int kb = k0 + grp * KB, b0, b1;                 // this group's tile, pages of it and of the next
+    if (threadIdx.x == 0) again = 0;
+    if (nt > 0) {
+        pages(kb);
+        b0 = load(kb);
+        pages(kb + GR * KB);
+        stash(0, kb, b0);
+        b1 = load(kb + GR * KB);
+        pages(kb + 2 * GR * KB);
         __syncthreads();
+    }
+    for (int t0 = 0; t0 < nt; t0 += 2 * GR) {
+#pragma unroll
+        for (int buf = 0; buf < 2; buf++) {
+            if (t0 + buf * GR >= nt) break;
+            // the next tile's LDS writes and a later one's loads are issued before
+            // this one's products
+            stash(buf ^ 1, kb + GR * KB, b1);
+            const int b2 = load(kb + 2 * GR * KB);
+            if (t0 + buf * GR + grp < nt) tile_step(buf, kb, b0);
+            pages(kb + 3 * GR * KB);
+            b0 = b1;
+            b1 = b2;
+            kb += GR * KB;
+            __syncthreads();
+        }
     }
 
     // group 1's sums, brought to a common reference
