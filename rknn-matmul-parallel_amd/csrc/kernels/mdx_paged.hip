@@ -63,6 +63,13 @@ Paged paged(const MdxPagedCache* c, const MdxPagedBatch* b) {
     return p;
 }
 
+// A value of the batch's arrays, which no kernel writes, by a scalar load (the
+// compiler takes a vector load where the address is one that could be stored to).
+__device__ __forceinline__ int fixed(const int* a, size_t i) {
+    typedef __attribute__((address_space(4))) const int c_int;
+    return ((c_int*)a)[i];
+}
+
 // A request's new rows: [start, start + n) of the batch; base: the cache row of
 // the first (negative if the cache is shorter than they are).
 struct Req {
@@ -70,9 +77,9 @@ struct Req {
 };
 __device__ __forceinline__ Req req_of(const Paged& p, int r) {
     Req q;
-    q.start = min(max(p.q_start[r], 0), p.n_tokens);
-    q.n = max(min(p.q_start[r + 1], p.n_tokens) - q.start, 0);
-    q.base = max(p.kv_len[r], 0) - q.n;
+    q.start = min(max(fixed(p.q_start, r), 0), p.n_tokens);
+    q.n = max(min(fixed(p.q_start, r + 1), p.n_tokens) - q.start, 0);
+    q.base = max(fixed(p.kv_len, r), 0) - q.n;
     return q;
 }
 
@@ -539,6 +546,14 @@ __device__ __forceinline__ uint2 lds_read_tr(const uint16_t* p) {
     const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
     return __builtin_bit_cast(uint2, v);
 }
+// What a row's 16-byte chunk numbers are XORed with in LDS, by the row number
+// mod 16.  A read of K takes one chunk of each of 32 rows: all values occur.  A
+// transposing read of V takes four neighbouring chunks of rows 0-3 and 4-7 (or 8-11
+// and 12-15): consecutive rows differ in the bits above the lowest two.
+template <int HD>
+__device__ __forceinline__ int lds_swap(int row) {
+    return HD == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
 // The other 32 lanes' value.
 __device__ __forceinline__ float half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -600,12 +615,14 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     constexpr int GR = HD == 256 ? 1 : 2;           // groups of four waves
     constexpr int KB = HD == 256 ? 32 : 64;         // keys per tile
     constexpr int CH = HD / 8;                      // 16-byte chunks per row
-    constexpr int SW = CH < 16 ? CH - 1 : 15;       // rows whose chunks are permuted apart
     constexpr int DS = HD / 16, DT = HD / 32, KT = KB / 32;
-    constexpr int U = KB * CH / 256;                // chunks per thread and tile
-    constexpr int RPU = 256 / CH;                   // rows per round of chunks
+    constexpr int U = KB * CH / 256;                // 16-byte loads per thread and tile
+    constexpr int RPU = 256 / CH, RPW = 64 / CH;    // rows per round of loads, of a group and of a wave
     constexpr int TN = KB * HD;                     // values per tile
-    __shared__ __attribute__((aligned(16))) uint16_t lds[GR * 2 * 2 * TN];
+    // tiles of even and odd numbers apart: the compiler then knows that a tile on
+    // its way to LDS is not the one that is read
+    __shared__ __attribute__((aligned(16))) uint16_t k_even[GR * TN], k_odd[GR * TN], v_even[GR * TN], v_odd[GR * TN];
+    __shared__ float mg_ref[GR * 128], mg_sum[GR * 128];
     __shared__ int again;
 
     const Paged& p = a.p;
@@ -669,70 +686,81 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         for (int s = 0; s < DS; s++) qf[s] = *reinterpret_cast<const u32x4_t*>(qr + 16 * s);
     }
 
-    // Staging: round i of this thread is chunk tid % CH of row tid / CH + i RPU; a
-    // wave's rows of a round lie in 16 keys, so in one page.  A tile's page numbers
-    // are read two tiles before its rows are requested, and these one tile before
-    // they go to LDS, so that nothing waits for what it has just asked for.
+    // Tiles go from the pages straight into LDS.  Round i of a wave is RPW rows of
+    // it, which lie in 16 keys and so in one page; LDS takes the lanes' chunks in
+    // order, so a lane asks for the chunk that belongs in its place.  Keys past the
+    // last one that the block sees repeat it; keys on pages that do not exist are
+    // rows of page 0.  Both are masked.
     const int* table = p.table + (size_t)r * p.max_pages;
     const int pmask = (1 << p.shift) - 1;
     const int srow = tid / CH, sch = tid % CH;
     constexpr int NG = KB / 16;                     // 16-key groups of a tile
-    int pg[NG];
+    const bool whole = (1 << p.shift) >= KB;        // a tile lies in one page
+    typedef int i4_t __attribute__((ext_vector_type(4)));
+    i4_t pgv, pgk, pgn;                             // page numbers of the next V and K tiles, and of one more
     auto pages = [&](int kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < NG; u++) pg[u] = table[min(kb + 16 * u, k1 - 1) >> p.shift];
-    };
-    // (wrow + i RPU) / 16
-    auto group = [&](int i) __attribute__((always_inline)) -> int {
-        return CH == 8 ? 2 * i + (wave >> 1) : (CH == 16 ? i : i >> 1);
-    };
-    u32x4_t kr[U], vr[U];
-    const size_t head = (size_t)kvh << p.shift;
-    // requests the tile whose page numbers are in pg; returns which of them exist
-    auto load = [&](int kb) __attribute__((always_inline)) -> int {
-        int bits = 0;
-#pragma unroll
-        for (int u = 0; u < NG; u++) {
-            const bool ok = kb + 16 * u < k1 && (unsigned)pg[u] < (unsigned)p.n_pages;
-            bits |= ok ? 1 << u : 0;
-            pg[u] = ok ? pg[u] : 0;
+        pgn = i4_t(fixed(table, min(kb, kend - 1) >> p.shift));
+        if (!whole) {
+            pgn.y = fixed(table, min(kb + 16, kend - 1) >> p.shift);
+            if constexpr (NG == 4) {
+                pgn.z = fixed(table, min(kb + 32, kend - 1) >> p.shift);
+                pgn.w = fixed(table, min(kb + 48, kend - 1) >> p.shift);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < U; i++) {
-            const int u = group(i);
-            const int page = CH == 8 ? ((wave >> 1) ? pg[2 * i + 1] : pg[2 * i]) : pg[CH == 16 ? i : i >> 1];
-            const size_t base = ((((size_t)page * p.nkv) << p.shift) + head + ((kb + 16 * u) & pmask)) * HD;
-            const unsigned at = ((srow + i * RPU) & 15) * HD + 8 * sch;
-            kr[i] = *reinterpret_cast<const u32x4_t*>(p.kp + base + at);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(p.vp + base + at);
-        }
-        return bits;
     };
-    uint16_t* const kbuf = lds + grp * 4 * TN;      // [2][K tile, V tile]
-    auto stash = [&](int buf, int kb, int bits) __attribute__((always_inline)) {
-        if (kb + KB > kend || bits != (1 << NG) - 1) {
+    auto turn_pages = [&]() __attribute__((always_inline)) {
+        pgv = pgk;
+        pgk = pgn;
+    };
+    auto there = [&](int page) __attribute__((always_inline)) -> bool { return (unsigned)page < (unsigned)p.n_pages; };
+    auto exist = [&]() __attribute__((always_inline)) -> int {  // which of the K tile's groups do
+        const int bits = (there(pgk.x) ? 1 : 0) | (there(pgk.y) ? 2 : 0);
+        return NG == 4 ? bits | (there(pgk.z) ? 4 : 0) | (there(pgk.w) ? 8 : 0) : bits;
+    };
+    // byte offset of this lane's chunk in a whole tile; rounds V apart have the
+    // same chunks, V RPU rows on
+    constexpr int V = RPU % 16 ? 2 : 1;
+    unsigned goes[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) goes[i] = 2 * ((srow + i * RPU) * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU)));
+    auto load = [&](const uint16_t* src, i4_t pg, uint16_t* dst, int kb) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(1))) const void gptr_t;
+        typedef __attribute__((address_space(3))) void lptr_t;
+        auto base = [&](int page, int key) __attribute__((always_inline)) -> const char* {
+            return reinterpret_cast<const char*>(src + ((((size_t)(there(page) ? page : 0) * p.nkv + kvh) << p.shift) + (key & pmask)) * HD);
+        };
+        if (kb >= k1) return;
+        if (whole && kb + KB <= kend) {
+            const char* at = base(pg.x, kb);
 #pragma unroll
             for (int i = 0; i < U; i++)
-                if (!((bits >> group(i)) & 1) || kb + srow + i * RPU >= kend) vr[i] = u32x4_t{0u, 0u, 0u, 0u};
+                __builtin_amdgcn_global_load_lds((gptr_t*)(at + i / V * (V * RPU * HD * 2) + goes[i % V]),
+                                                 (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
+            return;
         }
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const int row = srow + i * RPU, at = row * HD + 8 * (sch ^ (row & SW));
-            *reinterpret_cast<u32x4_t*>(kbuf + buf * 2 * TN + at) = kr[i];
-            *reinterpret_cast<u32x4_t*>(kbuf + buf * 2 * TN + TN + at) = vr[i];
+            // this round's 16 keys: 2 i + wave / 2, i or i / 2
+            const int even = CH == 8 ? 2 * i : (CH == 16 ? i : i >> 1);
+            const int page = CH == 8 && (wave >> 1) ? pg[(even + 1) & 3] : pg[even];
+            const int key = min(kb + 16 * (even + (CH == 8 ? wave >> 1 : 0)), (kend - 1) & ~15);
+            const unsigned row = min((srow + i * RPU) & 15, kend - 1 - key);
+            const unsigned at = 2 * (row * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU)));
+            __builtin_amdgcn_global_load_lds((gptr_t*)(base(page, key) + at),
+                                             (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
         }
     };
     // where this lane reads: K rows c32 (+ 32 kt), chunk 2 d + hi; V rows 4 hi + ..
     // (+ 16 kk, + 8), four values of column 32 d + ..
     int kat[DS], vat[DT][2];
 #pragma unroll
-    for (int d = 0; d < DS; d++) kat[d] = grp * 4 * TN + c32 * HD + 8 * ((2 * d + hi) ^ (c32 & SW));
+    for (int d = 0; d < DS; d++) kat[d] = grp * TN + c32 * HD + 8 * ((2 * d + hi) ^ lds_swap<HD>(c32));
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int key = 8 * e + 4 * hi + ((lane & 15) >> 2), col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            vat[d][e] = grp * 4 * TN + TN + key * HD + 8 * ((col >> 3) ^ (key & SW)) + (col & 7);
+            vat[d][e] = grp * TN + key * HD + 8 * ((col >> 3) ^ lds_swap<HD>(key)) + (col & 7);
         }
 
     float16_t o[DT];
@@ -742,48 +770,46 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float ref = -INFINITY, l = 0.0f;
     bool seen = false;
+    float16_t s[KT];
+    u32x4_t pf[KB / 16];
 
-    auto tile_step = [&](int buf, int kb, int bits) __attribute__((always_inline)) {
-        const uint16_t* ks = lds + buf * 2 * TN;
-        float16_t s[KT];
-        u32x4_t kf[2][DS];
+    // The products read their fragments from LDS ahead: the first ones before the
+    // phase begins, the others one product set before they are needed.
+    u32x4_t kf[DS];
+    uint2 vf[2][DT][2];
+    auto kload = [&](const uint16_t* ks, int kt, int d) __attribute__((always_inline)) {
+        kf[d] = *reinterpret_cast<const u32x4_t*>(ks + kat[d] + 32 * kt * HD);
+    };
+    auto vload = [&](const uint16_t* vs, int kk, int d) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < DS; d++) kf[0][d] = *reinterpret_cast<const u32x4_t*>(ks + kat[d]);
+        for (int e = 0; e < 2; e++) vf[kk & 1][d][e] = lds_read_tr(vs + vat[d][e] + 16 * kk * HD);
+    };
+    // s = scores of the K tile (its first fragments are in kf)
+    auto scores = [&](const uint16_t* ks) __attribute__((always_inline)) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
             for (int i = 0; i < 16; i++) s[kt][i] = 0.0f;
 #pragma unroll
             for (int d = 0; d < DS; d++) {
-                s[kt] = mfma32(T(), kf[kt & 1][d], qf[d], s[kt]);
-                if (kt + 1 < KT) kf[(kt + 1) & 1][d] = *reinterpret_cast<const u32x4_t*>(ks + kat[d] + 32 * (kt + 1) * HD);
+                s[kt] = mfma32(T(), kf[d], qf[d], s[kt]);
+                if (kt + 1 < KT) kload(ks, kt + 1, d);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                if (kt + 1 < KT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
-        uint2 vf[2][DT][2];
-        auto vload = [&](int kk) __attribute__((always_inline)) {
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) vf[kk & 1][d][e] = lds_read_tr(ks + vat[d][e] + 16 * kk * HD);
-        };
-        vload(0);
-        // fragments ahead of the products that take them
-        __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
-#pragma unroll
-        for (int i = 0; i < DS * (KT - 1); i++) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
+    };
+    // pf = probabilities of s (keys kb ..), and what becomes of the sums so far
+    auto softmax = [&](int kb, int bits) __attribute__((always_inline)) {
         if (kb + KB > vmin || bits != (1 << NG) - 1) {
             // pages that do not exist, and keys that some row does not see
+            const int end = vis - kb - 4 * hi;
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = 32 * kt + 8 * (i >> 2) + (i & 3);     // + 4 hi
-                    if (!((bits >> (key >> 4)) & 1) || kb + key + 4 * hi >= vis) s[kt][i] = -INFINITY;
+                    if (!((bits >> (key >> 4)) & 1) || key >= end) s[kt][i] = -INFINITY;
                     else seen = true;
                 }
         } else {
@@ -821,8 +847,7 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         }
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < KB / 16; kk++) {
-            u32x4_t pf;
+        for (int kk = 0; kk < KB / 16; kk++)
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 float x[2];
@@ -831,60 +856,114 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
                     x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][8 * (kk & 1) + 2 * w + e], a.c, off));
                     l4[2 * (w & 1) + e] = l4[2 * (w & 1) + e] + x[e];
                 }
-                pf[w] = pack16<T>(x[0], x[1]);
+                pf[kk][w] = pack16<T>(x[0], x[1]);
             }
-            if (kk + 1 < KB / 16) vload(kk + 1);
+        l = l + ((l4[0] + l4[1]) + (l4[2] + l4[3]));
+    };
+    // o += V tile . pf (its first fragments are in vf[0]); then the first of ks
+    auto values = [&](const uint16_t* vs, const uint16_t* ks) __attribute__((always_inline)) {
+        constexpr int KK = KB / 16, KPD = (DS + DT - 1) / DT;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 const uint2 v0 = vf[kk & 1][d][0], v1 = vf[kk & 1][d][1];
-                o[d] = mfma32(T(), u32x4_t{v0.x, v0.y, v1.x, v1.y}, pf, o[d]);
+                o[d] = mfma32(T(), u32x4_t{v0.x, v0.y, v1.x, v1.y}, pf[kk], o[d]);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                if (kk + 1 < KK) {
+                    vload(vs, kk + 1, d);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                } else {
+#pragma unroll
+                    for (int x = KPD * d; x < KPD * (d + 1) && x < DS; x++) kload(ks, 0, x);
+                    __builtin_amdgcn_sched_group_barrier(0x100, KPD, 0);
+                }
             }
-        }
-        l = l + ((l4[0] + l4[1]) + (l4[2] + l4[3]));
     };
 
-    const int nt = (k1 - k0 + KB - 1) / KB;
-    int kb = k0 + grp * KB, b0, b1;                 // this group's tile, pages of it and of the next
+    // A group's phases: the softmax of tile t; then the products V of t and K of
+    // t + 1.  The other group is one phase off, so that the SIMDs' matrix and
+    // vector units are asked for by one of the two at a time.  Rows of t + 1 (V)
+    // and t + 2 (K) are requested at the beginning of the first phase.
+    const int nt = (k1 - k0 + KB - 1) / KB, steps = (nt + GR - 1) / GR;
+    int kb = k0 + grp * KB;                         // this group's tile
     if (threadIdx.x == 0) again = 0;
+    int bits = 0, bits1 = 0, bits2;                 // groups of 16 keys that exist: this tile, the next ones
+    // what a wave has requested is in LDS once it has waited for it
+    auto arrived = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
     if (nt > 0) {
         pages(kb);
-        b0 = load(kb);
+        turn_pages();
         pages(kb + GR * KB);
-        stash(0, kb, b0);
-        b1 = load(kb + GR * KB);
+        bits = exist();
+        load(p.kp, pgk, k_even, kb);
+        load(p.vp, pgk, v_even, kb);
+        turn_pages();
         pages(kb + 2 * GR * KB);
-        __syncthreads();
-    }
-    for (int t0 = 0; t0 < nt; t0 += 2 * GR) {
+        bits1 = exist();
+        load(p.kp, pgk, k_odd, kb + GR * KB);
+        turn_pages();
+        arrived();
+        if (grp < nt) {
 #pragma unroll
-        for (int buf = 0; buf < 2; buf++) {
-            if (t0 + buf * GR >= nt) break;
-            // the next tile's LDS writes and a later one's loads are issued before
-            // this one's products
-            stash(buf ^ 1, kb + GR * KB, b1);
-            const int b2 = load(kb + 2 * GR * KB);
-            if (t0 + buf * GR + grp < nt) tile_step(buf, kb, b0);
+            for (int d = 0; d < DS; d++) kload(k_even, 0, d);
+            scores(k_even);
+        }
+        if (grp == 1) __syncthreads();
+    }
+    for (int t0 = 0; t0 < steps; t0 += 2) {
+#pragma unroll
+        for (int odd = 0; odd < 2; odd++) {
+            const int t = (t0 + odd) * GR + grp;
+            if (t0 + odd >= steps) break;
+            load(p.vp, pgv, odd ? v_even : v_odd, kb + GR * KB);
+            load(p.kp, pgk, odd ? k_odd : k_even, kb + 2 * GR * KB);
+            bits2 = exist();
             pages(kb + 3 * GR * KB);
-            b0 = b1;
-            b1 = b2;
+            if (t < nt) {
+                softmax(kb, bits);
+#pragma unroll
+                for (int d = 0; d < DT; d++) vload(odd ? v_odd : v_even, 0, d);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            // (after the last tile: the scores of one that nobody asks for)
+            if (t < nt) {
+                values(odd ? v_odd : v_even, odd ? k_even : k_odd);
+                scores(odd ? k_even : k_odd);
+            }
+            turn_pages();
+            bits = bits1;
+            bits1 = bits2;
             kb += GR * KB;
-            __syncthreads();
+            arrived();
         }
     }
+    if (GR == 2 && grp == 0 && nt > 0) __syncthreads();
+    __syncthreads();
 
     // group 1's sums, brought to a common reference
     l = half_sum(l);
     if (ref == -INFINITY && l == l) l = seen ? 1.0f : 0.0f;
-    float* const mg = reinterpret_cast<float*>(lds);
-    static_assert(GR == 1 || (16 * DT + 2) * 256 * 4 <= (int)sizeof lds, "the merge fits the tiles");
+    // (a quarter of the lanes' outputs in each of the tiles' arrays)
+    static_assert(GR == 1 || 16 * DT * 256 * 4 <= 4 * (int)sizeof k_even, "the merge fits the tiles");
+    float* const part[4] = {reinterpret_cast<float*>(k_even), reinterpret_cast<float*>(k_odd),
+                            reinterpret_cast<float*>(v_even), reinterpret_cast<float*>(v_odd)};
+    constexpr int PER = 16 * DT / 4;               // values per lane and array
     if (GR == 2) {
         if (grp == 1) {
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) mg[(16 * d + i) * 256 + tid] = o[d][i];
-            mg[16 * DT * 256 + tid] = ref;
-            mg[(16 * DT + 1) * 256 + tid] = l;
+                for (int i = 0; i < 16; i++) part[(16 * d + i) / PER][(16 * d + i) % PER * 256 + tid] = o[d][i];
+            if (hi == 0) {
+                mg_ref[32 * wave + c32] = ref;
+                mg_sum[32 * wave + c32] = l;
+            }
         }
         __syncthreads();
     }
@@ -892,12 +971,13 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     bool redo = false;
     if (grp == 0) {
         if (GR == 2) {
-            const float ref1 = mg[16 * DT * 256 + tid], l1 = mg[(16 * DT + 1) * 256 + tid], top = fmaxf(ref, ref1);
+            const float ref1 = mg_ref[32 * wave + c32], l1 = mg_sum[32 * wave + c32], top = fmaxf(ref, ref1);
             const float w0 = ref_weight(ref, top, a.c), w1 = ref_weight(ref1, top, a.c);
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * w0 + mg[(16 * d + i) * 256 + tid] * w1;
+                for (int i = 0; i < 16; i++)
+                    o[d][i] = o[d][i] * w0 + part[(16 * d + i) / PER][(16 * d + i) % PER * 256 + tid] * w1;
             l = l * w0 + l1 * w1;
             ref = top;
         }
