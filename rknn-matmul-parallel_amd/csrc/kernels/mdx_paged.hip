@@ -1115,9 +1115,17 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
 
 // ---- received weight ---------------------------------------------------------------
 //
-// A wave owns 16 keys of one KV head, whose rows stay in registers as the matrix
-// operand, and goes over the query rows that see them, 16 at a time; nobody else
-// adds to those keys, so the sums have one order.
+// The keys are what is owned: nobody else adds to a workgroup's keys, so their sums
+// have one order and need no atomics.  K rows stay in registers as the matrix
+// operand, query rows pass by.
+//   few query rows (a decoding step): a wave owns 16 keys and goes over all rows.
+//     Reading K is all there is to it: 32 requests of 2049 rows, 8 heads of 128, 18
+//     us, 4.7 TB/s.
+//   many (a chunk): a workgroup owns 64 keys (32 at 256 dimensions), its eight
+//     waves take every eighth tile of 32 rows, the next tile's rows on their way
+//     during the products of this one, and their sums are added in LDS in order.
+//     515 rows over 4000, 8 heads over 4 of 64, two requests: 36 -> XX us against
+//     the other form, which waits for each tile's rows.
 struct MassArgs {
     Paged p;
     const uint16_t* q;
@@ -1125,6 +1133,11 @@ struct MassArgs {
     float scale;
     const float* lse;
 };
+
+// The weight of score s.
+__device__ __forceinline__ float weight(float s, float scale, float lse) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale, -lse) * kLog2e);
+}
 
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
@@ -1138,7 +1151,7 @@ __global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
     const int kend = min(q.base + n, p.limit);
     const int kb = 64 * blockIdx.x + 16 * wave;
     if (rows == 0 || kb >= kend) return;
-    const int pg = p.table[(size_t)r * p.max_pages + (kb >> p.shift)];
+    const int pg = fixed(p.table, (size_t)r * p.max_pages + (kb >> p.shift));
     if ((unsigned)pg >= (unsigned)p.n_pages) return;
     const size_t row = (((size_t)pg * p.nkv + kvh) << p.shift) + (kb & ((1 << p.shift) - 1));
     u32x4_t kf[DS];
@@ -1156,10 +1169,7 @@ __global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
         const float ls = a.lse[(size_t)tok * p.nq + h];
         const int vis = R < rows && ls != -INFINITY ? min(q.base + i + 1, p.limit) : 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale, -ls) * kLog2e);
-            sum[e] = sum[e] + (kb + 4 * g + e < vis ? w : 0.0f);
-        }
+        for (int e = 0; e < 4; e++) sum[e] = sum[e] + (kb + 4 * g + e < vis ? weight(s[e], a.scale, ls) : 0.0f);
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) sum[e] = row_sum16(sum[e]);
@@ -1167,6 +1177,103 @@ __global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
         const float add = c16 == 0 ? sum[0] : c16 == 1 ? sum[1] : c16 == 2 ? sum[2] : sum[3];
         p.mass[row + 4 * g + c16] += add;
     }
+}
+
+constexpr int kMassRows = 32;          // query rows up to which the first form is taken
+constexpr int kMassWaves = 8;
+
+template <int HD, class T>
+__global__ __launch_bounds__(64 * kMassWaves, 2) void k_paged_mass_chunk(MassArgs a) {
+    constexpr int DS = HD / 16, KT = HD == 256 ? 1 : 2, KB = 32 * KT;
+    __shared__ float part[kMassWaves][KB];
+    const Paged& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int hi = lane >> 5, c32 = lane & 31;
+    const int r = blockIdx.z, kvh = blockIdx.y, kb = KB * blockIdx.x;
+    const Req q = req_of(p, r);
+    const int n = min(q.n, p.max_q), rows = n * p.G;
+    const int kend = min(q.base + n, p.limit);
+    if (rows == 0 || kb >= kend) return;
+
+    // K rows (of page 0 where a page does not exist: not written below)
+    u32x4_t kf[KT][DS];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) {
+        const long long at = pool_row(p, r, kvh, min(kb + 32 * kt + c32, kend - 1));
+        const uint16_t* kp = p.kp + (at < 0 ? 0 : at) * HD + 8 * hi;
+#pragma unroll
+        for (int d = 0; d < DS; d++) kf[kt][d] = *reinterpret_cast<const u32x4_t*>(kp + 16 * d);
+    }
+    float16_t sum[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum[kt][i] = 0.0f;
+
+    u32x4_t qn[DS];
+    float ln;
+    int vn;                                         // keys that this lane's row of the next tile sees
+    auto load = [&](int t0) __attribute__((always_inline)) {
+        const int R = t0 + c32, Rc = min(R, rows - 1), i = Rc / p.G;
+        const int tok = q.start + i, h = kvh * p.G + Rc % p.G;
+        const uint16_t* qr = a.q + (size_t)tok * a.q_stride + (size_t)h * HD + 8 * hi;
+#pragma unroll
+        for (int d = 0; d < DS; d++) qn[d] = *reinterpret_cast<const u32x4_t*>(qr + 16 * d);
+        ln = a.lse[(size_t)tok * p.nq + h];
+        vn = R < rows ? min(q.base + i + 1, p.limit) : 0;
+    };
+    const int first = max(kb - q.base, 0) * p.G / 32;     // the first tile with a row that sees key kb
+    int t0 = 32 * (first + wave);
+    load(t0);
+    for (; t0 < rows; t0 += 32 * kMassWaves) {
+        u32x4_t qf[DS];
+#pragma unroll
+        for (int d = 0; d < DS; d++) qf[d] = qn[d];
+        const float ls = ln;
+        const int vis = ls == -INFINITY ? 0 : vn;
+        load(t0 + 32 * kMassWaves);
+        float16_t s[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[kt][i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DS; d++) s[kt] = mfma32(T(), kf[kt][d], qf[d], s[kt]);
+        }
+        const bool edge = __any(vis < kb + KB);
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[kt][i] = weight(s[kt][i], a.scale, ls);
+        if (edge) {
+            const int end = vis - kb - 4 * hi;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (32 * kt + 8 * (i >> 2) + (i & 3) >= end) s[kt][i] = 0.0f;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) sum[kt] += s[kt];
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v = row_sum16(sum[kt][i]);
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            if (c32 == 0) part[wave][32 * kt + 8 * (i >> 2) + 4 * hi + (i & 3)] = v;
+        }
+    __syncthreads();
+    const int key = threadIdx.x;
+    if (key >= KB || kb + key >= kend) return;
+    const long long at = pool_row(p, r, kvh, kb + key);
+    if (at < 0) return;
+    float add = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMassWaves; w++) add = add + part[w][key];
+    p.mass[at] += add;
 }
 
 // ---- eviction -------------------------------------------------------------------------
@@ -1477,7 +1584,11 @@ void attn_launch(const AttnArgs& a, const Plan& s, hipStream_t st) {
 
 template <int HD, class T>
 void mass_launch(const MassArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((k_paged_mass<HD, T>), dim3(cdiv(a.p.limit, 64), a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
+    if ((long long)a.p.max_q * a.p.G <= kMassRows)
+        hipLaunchKernelGGL((k_paged_mass<HD, T>), dim3(cdiv(a.p.limit, 64), a.p.nkv, a.p.n_req), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_paged_mass_chunk<HD, T>), dim3(cdiv(a.p.limit, HD == 256 ? 32 : 64), a.p.nkv, a.p.n_req),
+                           dim3(64 * kMassWaves), 0, s, a);
 }
 
 }  // namespace
