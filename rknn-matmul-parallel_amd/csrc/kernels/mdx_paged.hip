@@ -1121,8 +1121,8 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
 //   few query rows (a decoding step): a wave owns 16 keys and goes over all rows.
 //     Reading K is all there is to it: 32 requests of 2049 rows, 8 heads of 128, 18
 //     us, 4.7 TB/s.
-//   many (a chunk): a workgroup owns 64 keys (32 at 256 dimensions), its eight
-//     waves take every eighth tile of 32 rows, the next tile's rows on their way
+//   many (a chunk): a workgroup owns 64 keys (32 at 256 dimensions), its four
+//     waves take every fourth tile of 32 rows, the next tile's rows on their way
 //     during the products of this one, and their sums are added in LDS in order.
 //     515 rows over 4000, 8 heads over 4 of 64, two requests: 36 -> XX us against
 //     the other form, which waits for each tile's rows.
@@ -1180,7 +1180,7 @@ __global__ __launch_bounds__(256) void k_paged_mass(MassArgs a) {
 }
 
 constexpr int kMassRows = 32;          // query rows up to which the first form is taken
-constexpr int kMassWaves = 8;
+constexpr int kMassWaves = 4;
 
 template <int HD, class T>
 __global__ __launch_bounds__(64 * kMassWaves, 2) void k_paged_mass_chunk(MassArgs a) {
@@ -1257,14 +1257,15 @@ __global__ __launch_bounds__(64 * kMassWaves, 2) void k_paged_mass_chunk(MassArg
         for (int kt = 0; kt < KT; kt++) sum[kt] += s[kt];
     }
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++)
+    for (int kt = 0; kt < KT; kt++) {
+        // over the 32 lanes of a half: lane l is left with value l / 2 of 16
+        float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v = row_sum16(sum[kt][i]);
-            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-            v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-            if (c32 == 0) part[wave][32 * kt + 8 * (i >> 2) + 4 * hi + (i & 3)] = v;
-        }
+        for (int i = 0; i < 16; i++) v[i] = sum[kt][i];
+        const float total = reduce_scatter<16, 32>(v, lane);
+        const int i = c32 >> 1;
+        if (!(lane & 1)) part[wave][32 * kt + 8 * (i >> 2) + 4 * hi + (i & 3)] = total;
+    }
     __syncthreads();
     const int key = threadIdx.x;
     if (key >= KB || kb + key >= kend) return;
