@@ -83,6 +83,13 @@ __device__ __forceinline__ Req req_of(const Paged& p, int r) {
     return q;
 }
 
+// Sum over the wave, the same in a scalar register.
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
 // The request of batch row t, by a whole wave: how many requests end at or
 // before it (n_req: the row is behind the last one).
 __device__ __forceinline__ int find_req(const Paged& p, int t, int lane) {
@@ -632,43 +639,36 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     const int kvh = blockIdx.x % p.nkv;
 
     // the request and the block of rows in it: the last ones (the longest) first
-    int r = -1, tile = 0;
-    {
-        int total = 0;
-        for (int pass = 0; pass < 2 && r < 0; pass++) {
-            const int want = total - 1 - (int)(blockIdx.x / p.nkv);
-            if (pass == 1 && want < 0) return;
-            int before = 0;
-            for (int j0 = 0; j0 < p.n_req; j0 += 64) {
-                int t = 0;
-                if (j0 + lane < p.n_req) {
-                    const Req q = req_of(p, j0 + lane);
-                    const int rows = min(q.n, p.max_q) * p.G;
-                    t = rows > a.short_max ? (rows + kRows - 1) / kRows : 0;
-                }
-                int incl = t;
+    auto blocks_of = [&](const Req& q) __attribute__((always_inline)) -> int {
+        const int rows = min(q.n, p.max_q) * p.G;
+        return rows > a.short_max ? (rows + kRows - 1) / kRows : 0;
+    };
+    Req q = {0, 0, 0};
+    int r = -1, tile = 0, total = 0;
+    for (int j0 = 0; j0 < p.n_req; j0 += 64) total += wave_total(j0 + lane < p.n_req ? blocks_of(req_of(p, j0 + lane)) : 0);
+    int want = total - 1 - (int)(blockIdx.x / p.nkv);
+    if (want < 0) return;
+    for (int j0 = 0; j0 < p.n_req && r < 0; j0 += 64) {
+        const Req mine = j0 + lane < p.n_req ? req_of(p, j0 + lane) : Req{0, 0, 0};
+        const int t = blocks_of(mine);
+        int upto = t;
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int y = __shfl_up(incl, o, kWave);
-                    if (lane >= o) incl += y;
-                }
-                if (pass == 1) {
-                    const unsigned long long hit = __ballot(before + incl > want);
-                    if (hit) {
-                        const int src = __builtin_ctzll(hit);
-                        r = j0 + src;
-                        tile = want - (before + __shfl(incl - t, src, kWave));
-                        break;
-                    }
-                }
-                before += __shfl(incl, 63, kWave);
-            }
-            total = before;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o, kWave);
+            if (lane >= o) upto += y;
+        }
+        const unsigned long long hit = __ballot(upto > want);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            r = j0 + src;
+            tile = want - __builtin_amdgcn_readlane(upto - t, src);
+            q.start = __builtin_amdgcn_readlane(mine.start, src);
+            q.n = __builtin_amdgcn_readlane(mine.n, src);
+            q.base = __builtin_amdgcn_readlane(mine.base, src);
+        } else {
+            want -= __builtin_amdgcn_readlane(upto, 63);
         }
     }
-    r = __builtin_amdgcn_readfirstlane(r);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    const Req q = req_of(p, r);
     const int rows = min(q.n, p.max_q) * p.G, row0 = tile * kRows;
     const int R = min(row0 + 32 * wave + c32, rows - 1);
     const int tok = q.start + R / p.G, hq = kvh * p.G + R % p.G;
@@ -729,13 +729,14 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         auto base = [&](int page, int key) __attribute__((always_inline)) -> const char* {
             return reinterpret_cast<const char*>(src + ((((size_t)(there(page) ? page : 0) * p.nkv + kvh) << p.shift) + (key & pmask)) * HD);
         };
+        auto go = [&](const char* from, int i) __attribute__((always_inline)) {
+            __builtin_amdgcn_global_load_lds((gptr_t*)from, (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
+        };
         if (kb >= k1) return;
         if (whole && kb + KB <= kend) {
             const char* at = base(pg.x, kb);
 #pragma unroll
-            for (int i = 0; i < U; i++)
-                __builtin_amdgcn_global_load_lds((gptr_t*)(at + i / V * (V * RPU * HD * 2) + goes[i % V]),
-                                                 (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
+            for (int i = 0; i < U; i++) go(at + i / V * (V * RPU * HD * 2) + goes[i % V], i);
             return;
         }
 #pragma unroll
@@ -745,9 +746,7 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
             const int page = CH == 8 && (wave >> 1) ? pg[(even + 1) & 3] : pg[even];
             const int key = min(kb + 16 * (even + (CH == 8 ? wave >> 1 : 0)), (kend - 1) & ~15);
             const unsigned row = min((srow + i * RPU) & 15, kend - 1 - key);
-            const unsigned at = 2 * (row * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU)));
-            __builtin_amdgcn_global_load_lds((gptr_t*)(base(page, key) + at),
-                                             (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
+            go(base(page, key) + 2 * (row * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU))), i);
         }
     };
     // where this lane reads: K rows c32 (+ 32 kt), chunk 2 d + hi; V rows 4 hi + ..
@@ -802,16 +801,21 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     // pf = probabilities of s (keys kb ..), and what becomes of the sums so far
     auto softmax = [&](int kb, int bits) __attribute__((always_inline)) {
         if (kb + KB > vmin || bits != (1 << NG) - 1) {
-            // pages that do not exist, and keys that some row does not see
+            // keys that some row does not see, and pages that do not exist
             const int end = vis - kb - 4 * hi;
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int key = 32 * kt + 8 * (i >> 2) + (i & 3);     // + 4 hi
-                    if (!((bits >> (key >> 4)) & 1) || key >= end) s[kt][i] = -INFINITY;
-                    else seen = true;
+                for (int i = 0; i < 16; i++) s[kt][i] = 32 * kt + 8 * (i >> 2) + (i & 3) < end ? s[kt][i] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < NG; u++) {
+                if ((bits >> u) & 1) {
+                    seen |= kb + 16 * u < vis;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[u >> 1][8 * (u & 1) + i] = -INFINITY;
                 }
+            }
         } else {
             seen = true;
         }
