@@ -629,8 +629,8 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     // tiles of even and odd numbers apart: the compiler then knows that a tile on
     // its way to LDS is not the one that is read
     __shared__ __attribute__((aligned(16))) uint16_t k_even[GR * TN], k_odd[GR * TN], v_even[GR * TN], v_odd[GR * TN];
-    __shared__ float mg_ref[GR * 128], mg_sum[GR * 128];
-    __shared__ int again;
+    __shared__ float mg_ref[GR * kRows], mg_sum[GR * kRows];
+    __shared__ int again, redo[kRows];
 
     const Paged& p = a.p;
     const int grp = GR == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -950,76 +950,104 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     if (GR == 2 && grp == 0 && nt > 0) __syncthreads();
     __syncthreads();
 
-    // group 1's sums, brought to a common reference
+    // The groups' sums, brought to a common reference: each group finishes half of
+    // the dims (at 256 dimensions the one group all) and leaves the other half in
+    // LDS for the other.
     l = half_sum(l);
     if (ref == -INFINITY && l == l) l = seen ? 1.0f : 0.0f;
-    // (a quarter of the lanes' outputs in each of the tiles' arrays)
-    static_assert(GR == 1 || 16 * DT * 256 * 4 <= 4 * (int)sizeof k_even, "the merge fits the tiles");
-    float* const part[4] = {reinterpret_cast<float*>(k_even), reinterpret_cast<float*>(k_odd),
-                            reinterpret_cast<float*>(v_even), reinterpret_cast<float*>(v_odd)};
-    constexpr int PER = 16 * DT / 4;               // values per lane and array
+    constexpr int DH = DT / GR;
+    static_assert(GR == 1 || DH * 16 * 256 * 4 <= (int)sizeof k_even, "the halves fit the tiles");
+    const int row = 32 * wave + c32;                // of the block
     if (GR == 2) {
         if (grp == 1) {
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) part[(16 * d + i) / PER][(16 * d + i) % PER * 256 + tid] = o[d][i];
-            if (hi == 0) {
-                mg_ref[32 * wave + c32] = ref;
-                mg_sum[32 * wave + c32] = l;
+            for (int d = 0; d < DH; d++) {
+                const float16_t x = o[d];
+                o[d] = o[d + DH];
+                o[d + DH] = x;
             }
         }
+        float4* const give = reinterpret_cast<float4*>(grp == 0 ? k_odd : k_even);
+#pragma unroll
+        for (int d = 0; d < DH; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                give[(4 * d + i / 4) * 256 + tid] =
+                    make_float4(o[d + DH][i], o[d + DH][i + 1], o[d + DH][i + 2], o[d + DH][i + 3]);
+        if (hi == 0) {
+            mg_ref[grp * kRows + row] = ref;
+            mg_sum[grp * kRows + row] = l;
+        }
+        if (threadIdx.x < kRows) redo[threadIdx.x] = 0;
+        __syncthreads();
+        const float ref1 = mg_ref[(grp ^ 1) * kRows + row], l1 = mg_sum[(grp ^ 1) * kRows + row], top = fmaxf(ref, ref1);
+        const float w0 = ref_weight(ref, top, a.c), w1 = ref_weight(ref1, top, a.c);
+        const float4* const take = reinterpret_cast<const float4*>(grp == 0 ? k_even : k_odd);
+#pragma unroll
+        for (int d = 0; d < DH; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 x = take[(4 * d + i / 4) * 256 + tid];
+                o[d][i] = o[d][i] * w0 + x.x * w1;
+                o[d][i + 1] = o[d][i + 1] * w0 + x.y * w1;
+                o[d][i + 2] = o[d][i + 2] * w0 + x.z * w1;
+                o[d][i + 3] = o[d][i + 3] * w0 + x.w * w1;
+            }
+        l = l * w0 + l1 * w1;
+        ref = top;
+    } else {
+        if (threadIdx.x < kRows) redo[threadIdx.x] = 0;
         __syncthreads();
     }
-    const bool rv = row0 + 32 * wave + c32 < rows;
-    bool redo = false;
-    if (grp == 0) {
-        if (GR == 2) {
-            const float ref1 = mg_ref[32 * wave + c32], l1 = mg_sum[32 * wave + c32], top = fmaxf(ref, ref1);
-            const float w0 = ref_weight(ref, top, a.c), w1 = ref_weight(ref1, top, a.c);
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    o[d][i] = o[d][i] * w0 + part[(16 * d + i) / PER][(16 * d + i) % PER * 256 + tid] * w1;
-            l = l * w0 + l1 * w1;
-            ref = top;
-        }
+    const bool rv = row0 + row < rows;
+    const size_t orow = (size_t)tok * p.nq + hq;
+    {
         float any = 0.0f;                  // NaN when an output is not finite
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DH; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) any = any + o[d][i] * 0.0f;
-        redo = rv && any != any && l == l;
-        if (redo) again = 1;
-        const size_t row = (size_t)tok * p.nq + hq;
-        if (rv && a.chunk_splits > 1) {
-            float* po = a.part_o + ((size_t)split * p.n_tokens * p.nq + row) * HD + 4 * hi;
+            for (int i = 0; i < 16; i++) any = __builtin_fmaf(o[d][i], 0.0f, any);
+        if (rv && any != any && l == l) {
+            redo[row] = 1;
+            again = 1;
+        }
+        const int col = 32 * DH * grp;
+        if (a.chunk_splits > 1) {
+            const size_t at = (size_t)split * p.n_tokens * p.nq + orow;
+            float* po = a.part_o + at * HD + col + 4 * hi;
+            if (rv) {
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DH; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4*>(po + 32 * d + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
-            if (hi == 0) a.part_ml[(size_t)split * p.n_tokens * p.nq + row] = make_float2(ref, l);
-        } else if (rv) {
-            uint16_t* dst = a.out + (size_t)tok * a.out_stride + (size_t)hq * HD + 4 * hi;
-            const float inv = 1.0f / l;
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4*>(po + 32 * d + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+                if (hi == 0 && grp == 0) a.part_ml[at] = make_float2(ref, l);
+            }
+        } else {
+            // eight dims a lane: the halves of a wave exchange every other four
+            uint16_t* dst = a.out + (size_t)tok * a.out_stride + (size_t)hq * HD + col + 8 * hi;
+            const float inv = ref == -INFINITY ? 0.0f : 1.0f / l;
+            const float none = row_result(0.0f, ref, l);
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+            for (int d = 0; d < DH; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    float x[4];
+                for (int i = 0; i < 16; i += 8) {
+                    uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = ref == -INFINITY ? row_result(0.0f, ref, l) : o[d][i + e] * inv;
-                    *reinterpret_cast<uint2*>(dst + 32 * d + 2 * i) = make_uint2(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]));
+                    for (int e = 0; e < 4; e++) {
+                        const float x = o[d][i + 2 * e] * inv, y = o[d][i + 2 * e + 1] * inv;
+                        w[e] = ref == -INFINITY ? pack16<T>(none, none) : pack16<T>(x, y);
+                    }
+                    const auto a0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+                    const auto a1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                    if (rv) *reinterpret_cast<uint4*>(dst + 32 * d + 2 * i) = make_uint4(a0[0], a1[0], a0[1], a1[1]);
                 }
-            if (a.lse && hi == 0) a.lse[row] = row_lse<T>(ref, l, a.scale);
+            if (rv && a.lse && hi == 0 && grp == 0) a.lse[orow] = row_lse<T>(ref, l, a.scale);
         }
     }
     __syncthreads();
     if (!again || grp != 0) return;
-    unsigned long long todo = __ballot(redo);
-    todo = (todo | (todo >> 32)) & 0xffffffffull;
+    unsigned long long todo = __ballot(redo[row] != 0) & 0xffffffffull;
     while (todo) {
         const int c = __builtin_ctzll(todo);
         todo &= todo - 1;
@@ -1027,14 +1055,14 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         float x[HD / 64], top, sum;
         row_again<HD, T>(p, r, kvh, a.q + (size_t)t2 * a.q_stride + (size_t)h2 * HD, a.c, k0,
                          min(k1, min(q.base + R2 / p.G + 1, p.limit)), x, &top, &sum);
-        const size_t row = (size_t)t2 * p.nq + h2;
+        const size_t row2 = (size_t)t2 * p.nq + h2;
 #pragma unroll
         for (int d = 0; d < HD / 64; d++) {
             const int at = HD / 64 * lane + d;
-            if (a.chunk_splits > 1) a.part_o[((size_t)split * p.n_tokens * p.nq + row) * HD + at] = x[d];
+            if (a.chunk_splits > 1) a.part_o[((size_t)split * p.n_tokens * p.nq + row2) * HD + at] = x[d];
             else a.out[(size_t)t2 * a.out_stride + (size_t)h2 * HD + at] = bits16<T>(row_result(x[d], top, sum));
         }
-        if (a.chunk_splits > 1 && lane == 0) a.part_ml[(size_t)split * p.n_tokens * p.nq + row] = make_float2(top, sum);
+        if (a.chunk_splits > 1 && lane == 0) a.part_ml[(size_t)split * p.n_tokens * p.nq + row2] = make_float2(top, sum);
     }
 }
 
