@@ -1545,6 +1545,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
 // How a batch is cut up.  Short requests: enough workgroups for the chip, but
 // splits of at least 256 keys; the others: splits only while there are fewer
 // blocks than CUs.
+constexpr int kCus = 256;
 struct Plan {
     int short_max;
     int tiles, splits, split_keys, short_rows;           // k_paged_attn (tiles 0: not launched)
@@ -1555,9 +1556,13 @@ Plan attn_plan(const Paged& p) {
     const int limit = p.limit > 0 ? p.limit : 1;
     const long long rows = (long long)p.max_q * p.G;
     s.short_rows = rows < kShort ? (int)rows : kShort;
-    // with as many rows as all requests can have, none is expected to be short (one
-    // that is all the same is taken along by k_paged_chunk)
-    s.short_max = rows > kShort && (long long)p.n_req * p.max_q <= p.n_tokens ? 0 : kShort;
+    // A batch with chunks whose blocks leave CUs free takes its short requests along
+    // in them: XX -> XX us for 24 requests, ten of them with chunks.
+    const long long chunk_blocks = (long long)p.n_tokens * p.G / kRows + p.n_req;
+    s.short_max = rows > kShort && chunk_blocks * p.nkv <= kCus ? 0 : kShort;
+    // With as many rows as all requests can have, none is expected to be short (one
+    // that is all the same is taken along).
+    if (rows > kShort && (long long)p.n_req * p.max_q <= p.n_tokens) s.short_max = 0;
     if (s.short_max) {
         s.tiles = cdiv(s.short_rows, 16);
         long long want = cdiv(1024, (long long)p.n_req * p.nkv * s.tiles);
@@ -1567,11 +1572,11 @@ Plan attn_plan(const Paged& p) {
         s.splits = cdiv(limit, s.split_keys);
     }
     if (rows > kShort) {
-        long long n = (long long)p.n_tokens * p.G / kRows + p.n_req;
+        long long n = chunk_blocks;
         const long long each = (long long)p.n_req * cdiv(rows, kRows);
         if (n > each) n = each;
         s.blocks = (int)n;
-        long long want = 256 / (n * p.nkv);
+        long long want = kCus / (n * p.nkv);
         const long long most = cdiv(limit, 512);
         want = want < 1 ? 1 : (want > most ? most : want);
         s.chunk_keys = cdiv(cdiv(limit, want), 128) * 128;
