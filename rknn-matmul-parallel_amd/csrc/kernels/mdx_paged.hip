@@ -287,12 +287,12 @@ __device__ __forceinline__ float ref_weight(float ref, float top, float c) {
     return ref == top ? 1.0f : __builtin_amdgcn_exp2f((ref - top) * c);
 }
 
-template <int HD, class T>
-__global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
+template <int HD, class T, int W>
+__global__ __launch_bounds__(64 * W, 2) void k_paged_attn(AttnArgs a) {
     constexpr int DS = HD / 32, DJ = HD / 16;
     constexpr int OS = HD + 4;                       // floats per row of the joined sums
-    __shared__ float osh[4 * 16 * OS];
-    __shared__ float msh[4][16], lsh[4][16];
+    __shared__ float osh[W * 16 * OS];
+    __shared__ float msh[W][16], lsh[W][16];
     const Paged& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int g = lane >> 4, c16 = lane & 15;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
         ref = -INFINITY;
         l = 0.0f;
         seen = false;
-        for (int kb = k0 + 32 * wave; kb < k1; kb += 128) {
+        for (int kb = k0 + 32 * wave; kb < k1; kb += 32 * W) {
             u32x4_t kf[2][DS];
             uint32_t vr[8][DJ / 2];
             size_t vrow[2];
@@ -468,7 +468,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
     }
     __syncthreads();
     {
-        const float top = fmaxf(fmaxf(msh[0][c16], msh[1][c16]), fmaxf(msh[2][c16], msh[3][c16]));
+        float top = msh[0][c16];
+#pragma unroll
+        for (int x = 1; x < W; x++) top = fmaxf(top, msh[x][c16]);
         const float w = ref_weight(ref, top, a.c);
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -478,23 +480,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
                     make_float4(o[j][i] * w, o[j + 1][i] * w, o[j + 2][i] * w, o[j + 3][i] * w);
     }
     __syncthreads();
-    // 16 threads per row, DJ values each
-    const int row = threadIdx.x >> 4, d0 = DJ * (threadIdx.x & 15);
+    // 4 W threads per row, DV values each
+    constexpr int DV = HD / (4 * W);
+    const int row = threadIdx.x / (4 * W), d0 = DV * (threadIdx.x % (4 * W));
     if (tile * 16 + row >= rows) return;
-    const float top = fmaxf(fmaxf(msh[0][row], msh[1][row]), fmaxf(msh[2][row], msh[3][row]));
-    float sum = 0.0f, v[DJ];
+    float top = msh[0][row];
 #pragma unroll
-    for (int j = 0; j < DJ; j++) v[j] = 0.0f;
+    for (int x = 1; x < W; x++) top = fmaxf(top, msh[x][row]);
+    float sum = 0.0f, v[DV];
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int j = 0; j < DV; j++) v[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
         sum = sum + lsh[w][row] * ref_weight(msh[w][row], top, a.c);
 #pragma unroll
-        for (int j = 0; j < DJ; j += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(osh + (w * 16 + row) * OS + d0 + j);
+        for (int j = 0; j < DV; j += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(osh + (w * 16 + row) * OS + d0 + j);
             v[j] += x.x;
             v[j + 1] += x.y;
-            v[j + 2] += x.z;
-            v[j + 3] += x.w;
         }
     }
     const int orow = tile * 16 + row, otok = q.start + orow / p.G, oh = kvh * p.G + orow % p.G;
@@ -502,13 +505,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(AttnArgs a) {
         const size_t at = (((size_t)split * p.n_req + r) * p.nkv + kvh) * a.short_rows + orow;
         float* po = a.short_o + at * HD + d0;
 #pragma unroll
-        for (int j = 0; j < DJ; j += 4) *reinterpret_cast<float4*>(po + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < DV; j += 2) *reinterpret_cast<float2*>(po + j) = make_float2(v[j], v[j + 1]);
         if (d0 == 0) a.short_ml[at] = make_float2(top, sum);
         return;
     }
     uint16_t* dst = a.out + (size_t)otok * a.out_stride + (size_t)oh * HD + d0;
 #pragma unroll
-    for (int j = 0; j < DJ; j += 2)
+    for (int j = 0; j < DV; j += 2)
         *reinterpret_cast<uint32_t*>(dst + j) = pack16<T>(row_result(v[j], top, sum), row_result(v[j + 1], top, sum));
     if (a.lse && d0 == 0) a.lse[(size_t)otok * p.nq + oh] = row_lse<T>(top, sum, a.scale);
 }
@@ -1070,16 +1073,16 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
 // ((split * n_req + r) * nkv + KV head) * short_rows + row of the short partials,
 // the others at split * n_tokens * nq + token * nq + head.
 template <int HD, class T, int W>
-__global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
-    constexpr int DL = HD / 64, RB = 4 / W;
-    __shared__ float osh[4][HD + 4];
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_paged_join(AttnArgs a) {
+    constexpr int DL = HD / 64;
+    __shared__ float osh[W][HD + 4];
     const Paged& p = a.p;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % W;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = W == 1 ? 0 : wave;
     const float* part_o;
     const float2* part_ml;
     size_t step;
     int t, h, kend, keys;
-    if (W == 4) {
+    if (W > 1) {
         // a block per short row
         const int r = blockIdx.z, kvh = blockIdx.y, R = blockIdx.x;
         const Req q = req_of(p, r);
@@ -1095,7 +1098,7 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a) {
         part_o = a.short_o + row * HD;
         part_ml = a.short_ml + row;
     } else {
-        const long long row = (long long)blockIdx.x * RB + wave / W;
+        const long long row = (long long)blockIdx.x * 4 + wave;
         if (row >= (long long)p.n_tokens * p.nq) return;
         t = (int)(row / p.nq);
         h = (int)(row % p.nq);
@@ -1546,9 +1549,12 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
 // splits of at least 256 keys; the others: splits only while there are fewer
 // blocks than CUs.
 constexpr int kCus = 256;
+constexpr int kOneSplit = 512;         // keys that one workgroup of eight waves takes, without a split
+constexpr int kSplitBlocks = 1024;
+constexpr int kWideJoin = 16;
 struct Plan {
     int short_max;
-    int tiles, splits, split_keys, short_rows;           // k_paged_attn (tiles 0: not launched)
+    int tiles, waves, splits, split_keys, short_rows;    // k_paged_attn (tiles 0: not launched)
     int blocks, chunk_splits, chunk_keys;                // k_paged_chunk (blocks 0: not launched)
 };
 Plan attn_plan(const Paged& p) {
@@ -1565,8 +1571,9 @@ Plan attn_plan(const Paged& p) {
     if (rows > kShort && (long long)p.n_req * p.max_q <= p.n_tokens) s.short_max = 0;
     if (s.short_max) {
         s.tiles = cdiv(s.short_rows, 16);
-        long long want = cdiv(1024, (long long)p.n_req * p.nkv * s.tiles);
-        const long long most = cdiv(limit, 256);
+        s.waves = limit <= kOneSplit ? 8 : 4;
+        long long want = cdiv(kSplitBlocks, (long long)p.n_req * p.nkv * s.tiles);
+        const long long most = s.waves == 8 ? 1 : cdiv(limit, 256);
         if (want > most) want = most;
         s.split_keys = cdiv(cdiv(limit, want), 128) * 128;
         s.splits = cdiv(limit, s.split_keys);
@@ -1612,12 +1619,16 @@ void attn_launch(const AttnArgs& a, const Plan& s, hipStream_t st) {
     if (s.blocks)
         hipLaunchKernelGGL((k_paged_chunk<HD, T>), dim3(s.blocks * a.p.nkv, s.chunk_splits), dim3(HD == 256 ? 256 : 512),
                            0, st, a);
-    if (s.tiles)
-        hipLaunchKernelGGL((k_paged_attn<HD, T>), dim3(s.splits, a.p.nkv * s.tiles, a.p.n_req), dim3(256), 0, st, a);
+    const dim3 grid(s.splits, a.p.nkv * s.tiles, a.p.n_req);
+    if (s.tiles && s.waves == 8) hipLaunchKernelGGL((k_paged_attn<HD, T, 8>), grid, dim3(512), 0, st, a);
+    else if (s.tiles) hipLaunchKernelGGL((k_paged_attn<HD, T, 4>), grid, dim3(256), 0, st, a);
     if (chunk_parts(a.p, s))
         hipLaunchKernelGGL((k_paged_join<HD, T, 1>), dim3(cdiv((long long)a.p.n_tokens * a.p.nq, 4)), dim3(256), 0, st, a);
-    if (short_parts(a.p, s))
-        hipLaunchKernelGGL((k_paged_join<HD, T, 4>), dim3(s.short_rows, a.p.nkv, a.p.n_req), dim3(256), 0, st, a);
+    if (short_parts(a.p, s)) {
+        const dim3 rows(s.short_rows, a.p.nkv, a.p.n_req);
+        if (s.splits > kWideJoin) hipLaunchKernelGGL((k_paged_join<HD, T, 16>), rows, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL((k_paged_join<HD, T, 4>), rows, dim3(256), 0, st, a);
+    }
 }
 
 template <int HD, class T>
