@@ -1381,78 +1381,89 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, int 
 }
 
 // One workgroup per (request, KV head).  A thread owns C consecutive rows (a
-// multiple of 4, so that four masses or positions are one load) and keeps their
-// keys in registers; C = 0: as many rows as it takes, read again in each pass.
+// multiple of 4, so that four masses or positions are one load), whose keys it
+// keeps in registers; C = 0: as many rows as it takes, read again in each pass.
 // The key of the last row that stays comes from a radix selection of 11, 11 and
 // 10 bits with histograms in LDS (the first digit is a mass's exponent and two
-// bits: 8 bits would put most rows into a few counters), then three scans over
-// the threads number the ties, the gaps and the rows that fill them.
+// bits: 8 bits would put most rows into a few counters; protected rows are counted
+// per thread).  One scan over the threads then tells each how many rows before its
+// own stay, and with that which gaps and fillers its rows are.
+// What bounds it is latency: the chain of loads (length, page, mass) and five
+// scans with their barriers.  4 requests x 8 heads of 16384 rows XX us, 32 x 8 of
+// 2049 XX us.
 template <int C>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
     __shared__ int hist[kSelBins];
-    __shared__ int sums[kSelWaves];
-    __shared__ int s_newest, s_digit, s_left;
+    __shared__ int sums[kSelWaves], sums2[kSelWaves];
+    __shared__ int s_newest, s_digit, s_left, s_first;
     const Paged& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x, r = blockIdx.y, item = r * p.nkv + h;
-    const int n = min(max(p.kv_len[r], 0), p.limit);
-    const bool copy = a.mass_out != p.mass || a.pos_out != p.pos;
-    if (n <= a.budget) {
-        if (tid == 0) a.count[item] = 0;
-        for (int j = tid; copy && j < n; j += kSelThreads) {
+    const int n = min(max(fixed(p.kv_len, r), 0), p.limit);
+    const bool over = n > a.budget;
+    // a row that stays keeps its place: all rows before the budget are copied, and
+    // what is moved into gaps then overwrites them
+    if (a.mass_out != p.mass || a.pos_out != p.pos)
+        for (int j = tid; j < min(n, a.budget); j += kSelThreads) {
             const long long at = pool_row(p, r, h, j);
             if (at < 0) continue;
             a.mass_out[at] = p.mass[at];
             a.pos_out[at] = p.pos[at];
         }
+    if (!over) {
+        if (tid == 0) a.count[item] = 0;
         return;
     }
     const int per = C ? C : cdiv4(n, kSelThreads);
-    const int j0 = tid * per, j1 = min(n, j0 + per);
+    const int j0 = min(tid * per, n), j1 = min(n, j0 + per);
 
-    // rows j..j+3 (j a multiple of 4): their place in the pool, or -1
-    auto place = [&](int j) -> long long { return j < j1 ? pool_row(p, r, h, j) : -1; };
-    if (tid == 0) s_newest = -1;
-    __syncthreads();
-    uint32_t key[C ? C : 1];
-    {
-        int newest = -1;
-        auto positions = [&](int j) __attribute__((always_inline)) {
-            const long long at = place(j);
-            int4 q = make_int4(-1, -1, -1, -1);
-            if (at >= 0) q = *reinterpret_cast<const int4*>(p.pos + at);
-            newest = max(newest, max(max(q.x, j + 1 < j1 ? q.y : -1), max(j + 2 < j1 ? q.z : -1, j + 3 < j1 ? q.w : -1)));
-        };
-        if constexpr (C != 0) {
-#pragma unroll
-            for (int c = 0; c < C; c += 4) positions(j0 + c);
-        } else {
-            for (int j = j0; j < j1; j += 4) positions(j);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, kWave));
-        if (lane == 0) atomicMax(&s_newest, newest);
-    }
-    __syncthreads();
-    const long long recent = (long long)s_newest - a.recent;
-    auto keys4 = [&](int j, uint32_t (&k)[4]) __attribute__((always_inline)) {
-        const long long at = place(j);
-        k[0] = k[1] = k[2] = k[3] = 0u;
+    // four rows from j (a multiple of 4): positions (-1 where there is no row), masses
+    auto rows4 = [&](int j, int4& q, float4& m) __attribute__((always_inline)) {
+        q = make_int4(-1, -1, -1, -1);
+        m = make_float4(0.f, 0.f, 0.f, 0.f);
+        const long long at = j < j1 ? pool_row(p, r, h, j) : -1;
         if (at < 0) return;
-        const float4 m = *reinterpret_cast<const float4*>(p.mass + at);
-        const int4 q = *reinterpret_cast<const int4*>(p.pos + at);
-        k[0] = q.x < a.sink || q.x > recent ? kProtected : mass_key(m.x);
-        k[1] = q.y < a.sink || q.y > recent ? kProtected : mass_key(m.y);
-        k[2] = q.z < a.sink || q.z > recent ? kProtected : mass_key(m.z);
-        k[3] = q.w < a.sink || q.w > recent ? kProtected : mass_key(m.w);
+        q = *reinterpret_cast<const int4*>(p.pos + at);
+        m = *reinterpret_cast<const float4*>(p.mass + at);
+        if (j + 1 >= j1) q.y = -1;
+        if (j + 2 >= j1) q.z = -1;
+        if (j + 3 >= j1) q.w = -1;
     };
+    if (tid == 0) s_newest = -1;
+    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
+    int4 q[C ? C / 4 : 1];
+    float4 m[C ? C / 4 : 1];
+    int newest = -1;
     if constexpr (C != 0) {
 #pragma unroll
-        for (int c = 0; c < C; c += 4) {
-            uint32_t k[4];
-            keys4(j0 + c, k);
+        for (int c = 0; c < C / 4; c++) rows4(j0 + 4 * c, q[c], m[c]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) key[c + e] = k[e];
+        for (int c = 0; c < C / 4; c++) newest = max(newest, max(max(q[c].x, q[c].y), max(q[c].z, q[c].w)));
+    } else {
+        for (int j = j0; j < j1; j += 4) {
+            rows4(j, q[0], m[0]);
+            newest = max(newest, max(max(q[0].x, q[0].y), max(q[0].z, q[0].w)));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, kWave));
+    __syncthreads();
+    if (lane == 0) atomicMax(&s_newest, newest);
+    __syncthreads();
+    const long long recent = (long long)s_newest - a.recent;
+    // (a row on a page that does not exist has the least key; its position is -1)
+    auto key_of = [&](int pos, float mass) __attribute__((always_inline)) -> uint32_t {
+        if (pos < 0) return 0u;
+        return pos < a.sink || pos > recent ? kProtected : mass_key(mass);
+    };
+    uint32_t key[C ? C : 1];
+    if constexpr (C != 0) {
+#pragma unroll
+        for (int c = 0; c < C / 4; c++) {
+            key[4 * c] = key_of(q[c].x, m[c].x);
+            key[4 * c + 1] = key_of(q[c].y, m[c].y);
+            key[4 * c + 2] = key_of(q[c].z, m[c].z);
+            key[4 * c + 3] = key_of(q[c].w, m[c].w);
         }
     }
     // f(row, key) for this thread's rows in order
@@ -1463,77 +1474,77 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
                 if (j0 + c < j1) f(j0 + c, key[c]);
         } else {
             for (int j = j0; j < j1; j += 4) {
-                uint32_t k[4];
-                keys4(j, k);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (j + e < j1) f(j + e, k[e]);
+                rows4(j, q[0], m[0]);
+                f(j, key_of(q[0].x, m[0].x));
+                if (j + 1 < j1) f(j + 1, key_of(q[0].y, m[0].y));
+                if (j + 2 < j1) f(j + 2, key_of(q[0].z, m[0].z));
+                if (j + 3 < j1) f(j + 3, key_of(q[0].w, m[0].w));
             }
         }
     };
 
-    int safe = 0, total;
-    each([&](int, uint32_t k) { safe += k == kProtected; });
-    sel_scan(safe, sums, lane, wave, &total);
     // kth: the least key that stays; left: how many rows of that key stay
-    uint32_t kth = kProtected;
-    int left = a.budget;
-    if (total < a.budget) {
-        left = a.budget - total;
-        uint32_t prefix = 0;
-        int top = 32;                     // bits above `top` are known
-        while (top > 0) {
-            const int bits = top > 11 ? 11 : top, shift = top - bits;
-            for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
-            __syncthreads();
-            each([&](int, uint32_t k) {
-                if (k != kProtected && (top == 32 || (k >> top) == (prefix >> top)))
-                    atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
-            });
-            __syncthreads();
-            // bins from the largest digit down, two per thread
-            const int b1 = kSelBins - 1 - 2 * tid, c1 = hist[b1], c0 = hist[b1 - 1];
-            int all;
-            const int above = sel_scan(c1 + c0, sums, lane, wave, &all);
-            if (above < left && above + c1 + c0 >= left) {
-                const bool second = above + c1 < left;
-                s_digit = second ? b1 - 1 : b1;
-                s_left = left - above - (second ? c1 : 0);
-            }
-            __syncthreads();
-            prefix |= (uint32_t)s_digit << shift;
-            left = s_left;
-            top = shift;
+    uint32_t kth = 0;
+    int left = a.budget, total;
+    for (int top = 32; top > 0;) {                  // bits from `top` up are known
+        const int bits = top > 11 ? 11 : top, shift = top - bits, last = (1 << bits) - 1;
+        int safe = 0;
+        each([&](int, uint32_t k) {
+            if (top < 32 && (k >> (top & 31)) != (kth >> (top & 31))) return;
+            if (k == kProtected) safe++;
+            else atomicAdd(&hist[(k >> shift) & last], 1);
+        });
+        if (safe) atomicAdd(&hist[last], safe);
+        __syncthreads();
+        // bins from the largest digit down, two per thread
+        const int b1 = kSelBins - 1 - 2 * tid, c1 = hist[b1], c0 = hist[b1 - 1];
+        const int above = sel_scan(c1 + c0, sums, lane, wave, &total);
+        if (above < left && above + c1 + c0 >= left) {
+            const bool second = above + c1 < left;
+            s_digit = second ? b1 - 1 : b1;
+            s_left = left - above - (second ? c1 : 0);
         }
-        kth = prefix;
+        hist[b1] = hist[b1 - 1] = 0;
+        __syncthreads();
+        kth |= (uint32_t)s_digit << shift;
+        left = s_left;
+        top = shift;
+        if (a.budget == 0) break;
     }
-    int ties = 0;
-    each([&](int, uint32_t k) { ties += k == kth; });
-    const int before = sel_scan(ties, sums, lane, wave, &total);
-    int tie = before, gaps = 0, fill = 0;
-    each([&](int j, uint32_t k) {
-        const bool stay = k > kth || (k == kth && tie++ < left);
-        gaps += !stay && j < a.budget;
-        fill += stay && j >= a.budget;
+    if (a.budget == 0) kth = kProtected, left = 0;  // (no digit is found: nothing stays)
+    int greater = 0, ties = 0;
+    each([&](int, uint32_t k) {
+        greater += k > kth;
+        ties += k == kth;
     });
-    int moves;
-    int g = sel_scan(gaps, sums, lane, wave, &total), f = sel_scan(fill, sums, lane, wave, &moves);
-    const size_t list = (size_t)item * a.most;
-    tie = before;
-    each([&](int j, uint32_t k) {
-        const bool stay = k > kth || (k == kth && tie++ < left);
-        if (!stay && j < a.budget) a.to[list + g++] = j;
-        if (stay && j >= a.budget) a.from[list + f++] = j;
-        if (stay && j < a.budget && copy) {
-            const long long at = pool_row(p, r, h, j);
-            if (at >= 0) {
-                a.mass_out[at] = p.mass[at];
-                a.pos_out[at] = p.pos[at];
-            }
+    int tie = sel_scan(ties, sums2, lane, wave, &total);
+    const int stay0 = sel_scan(greater, sums, lane, wave, &total) + min(tie, left);   // rows before j0 that stay
+    // rows before the budget that stay: its thread knows
+    {
+        int st = stay0, t = tie;
+        if (j0 <= a.budget && a.budget < j0 + per) {
+            each([&](int j, uint32_t k) { st += j < a.budget && (k > kth || (k == kth && t++ < left)); });
+            s_first = st;
         }
+    }
+    __syncthreads();
+    const int first = s_first;
+    const size_t list = (size_t)item * a.most;
+    int st = stay0;
+    each([&](int j, uint32_t k) {
+        const bool stay = k > kth || (k == kth && tie++ < left);
+        if (j < a.budget) {
+            if (!stay) a.to[list + j - st] = j;
+        } else if (stay) {
+            a.from[list + st - first] = j;
+        }
+        st += stay;
     });
+    const int moves = a.budget - first;
     if (tid == 0) a.count[item] = moves;
     if (!a.move_here) return;
+    // the lists and the copies above are there before a row is moved
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     move_rows(a, r, h, moves, 0, kSelThreads / (a.hd / 8));
 }
