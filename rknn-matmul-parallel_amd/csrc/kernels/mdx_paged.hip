@@ -1338,36 +1338,41 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 constexpr int kSelBins = 2048;
 constexpr int kSelMoves = 64;      // moves that the selecting workgroup makes itself
 
-// Sum over the threads before this one, and over all; `sums` is scratch.
-__device__ __forceinline__ int sel_scan(int v, int* sums, int lane, int wave, int* total) {
-    int incl = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(incl, o, kWave);
-        if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = incl;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kSelWaves; w++) {
-        const int s = sums[w];
-        before += w < wave ? s : 0;
-        all += s;
-    }
-    *total = all;
-    return before + incl - v;
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2, 3
+    return v;
 }
 
-// A thread's row moves; sources lie behind the budget and targets before it, so
-// no order is needed.  16 bytes per thread, hd / 8 threads per row.
-__device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, int count, int first, int step) {
+// Sums of two values over the threads before this one; `sums` is scratch that is
+// not in use.
+__device__ __forceinline__ int2 sel_scan(int x, int y, int2* sums, int lane, int wave) {
+    const int ix = wave_scan(x), iy = wave_scan(y);
+    if (lane == 63) sums[wave] = make_int2(ix, iy);
+    __syncthreads();
+    int2 before = make_int2(ix - x, iy - y);
+#pragma unroll
+    for (int w = 0; w < kSelWaves; w++) {
+        const int2 s = sums[w];
+        before.x += w < wave ? s.x : 0;
+        before.y += w < wave ? s.y : 0;
+    }
+    return before;
+}
+
+// Row moves by a workgroup; sources lie behind the budget and targets before it,
+// so no order is needed.  16 bytes per thread, hd / 8 threads per row.
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, const int* from, const int* to, int count,
+                                          int first, int step) {
     const Paged& p = a.p;
     const int per = a.hd / 8, c = threadIdx.x % per;
-    const size_t list = (size_t)(r * p.nkv + h) * a.most;
     for (int m = first + threadIdx.x / per; m < count; m += step) {
-        const long long src = pool_row(p, r, h, a.from[list + m]), dst = pool_row(p, r, h, a.to[list + m]);
+        const long long src = pool_row(p, r, h, from[m]), dst = pool_row(p, r, h, to[m]);
         if (src < 0 || dst < 0) continue;
         const uint4 k = *reinterpret_cast<const uint4*>(p.kp + src * a.hd + 8 * c);
         const uint4 v = *reinterpret_cast<const uint4*>(p.vp + src * a.hd + 8 * c);
@@ -1385,16 +1390,17 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, int 
 // keeps in registers; C = 0: as many rows as it takes, read again in each pass.
 // The key of the last row that stays comes from a radix selection of 11, 11 and
 // 10 bits with histograms in LDS (the first digit is a mass's exponent and two
-// bits: 8 bits would put most rows into a few counters; protected rows are counted
-// per thread).  One scan over the threads then tells each how many rows before its
+// bits: 8 bits would put most rows into a few counters; four copies of a counter,
+// by lane; protected rows are counted per thread).  One scan over the threads then tells each how many rows before its
 // own stay, and with that which gaps and fillers its rows are.
 // What bounds it is latency: the chain of loads (length, page, mass) and five
 // scans with their barriers.  4 requests x 8 heads of 16384 rows XX us, 32 x 8 of
 // 2049 XX us.
 template <int C>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
-    __shared__ int hist[kSelBins];
-    __shared__ int sums[kSelWaves], sums2[kSelWaves];
+    __shared__ int4 hist[kSelBins];
+    __shared__ int2 sums[4][kSelWaves];
+    __shared__ int lds_from[kSelMoves], lds_to[kSelMoves];
     __shared__ int s_newest, s_digit, s_left, s_first;
     const Paged& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1430,7 +1436,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
         if (j + 3 >= j1) q.w = -1;
     };
     if (tid == 0) s_newest = -1;
-    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
+    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = make_int4(0, 0, 0, 0);
     int4 q[C ? C / 4 : 1];
     float4 m[C ? C / 4 : 1];
     int newest = -1;
@@ -1485,40 +1491,43 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
 
     // kth: the least key that stays; left: how many rows of that key stay
     uint32_t kth = 0;
-    int left = a.budget, total;
-    for (int top = 32; top > 0;) {                  // bits from `top` up are known
-        const int bits = top > 11 ? 11 : top, shift = top - bits, last = (1 << bits) - 1;
+    int left = a.budget;
+    int* const mine = reinterpret_cast<int*>(hist) + (lane & 3);
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+        const int top = 32 - 11 * pass, bits = pass < 2 ? 11 : 10, shift = top - bits, last = (1 << bits) - 1;
         int safe = 0;
         each([&](int, uint32_t k) {
-            if (top < 32 && (k >> (top & 31)) != (kth >> (top & 31))) return;
+            if (pass > 0 && (k >> (top & 31)) != (kth >> (top & 31))) return;
             if (k == kProtected) safe++;
-            else atomicAdd(&hist[(k >> shift) & last], 1);
+            else atomicAdd(mine + 4 * ((k >> shift) & last), 1);
         });
-        if (safe) atomicAdd(&hist[last], safe);
+        if (safe) atomicAdd(mine + 4 * last, safe);
         __syncthreads();
         // bins from the largest digit down, two per thread
-        const int b1 = kSelBins - 1 - 2 * tid, c1 = hist[b1], c0 = hist[b1 - 1];
-        const int above = sel_scan(c1 + c0, sums, lane, wave, &total);
+        const int b1 = kSelBins - 1 - 2 * tid;
+        const int4 n1 = hist[b1], n0 = hist[b1 - 1];
+        const int c1 = (n1.x + n1.y) + (n1.z + n1.w), c0 = (n0.x + n0.y) + (n0.z + n0.w);
+        hist[b1] = hist[b1 - 1] = make_int4(0, 0, 0, 0);
+        const int above = sel_scan(c1 + c0, 0, sums[pass], lane, wave).x;
         if (above < left && above + c1 + c0 >= left) {
             const bool second = above + c1 < left;
             s_digit = second ? b1 - 1 : b1;
             s_left = left - above - (second ? c1 : 0);
         }
-        hist[b1] = hist[b1 - 1] = 0;
         __syncthreads();
         kth |= (uint32_t)s_digit << shift;
         left = s_left;
-        top = shift;
-        if (a.budget == 0) break;
     }
-    if (a.budget == 0) kth = kProtected, left = 0;  // (no digit is found: nothing stays)
+    if (a.budget == 0) kth = kProtected, left = 0;  // (no digit was found: nothing stays)
     int greater = 0, ties = 0;
     each([&](int, uint32_t k) {
         greater += k > kth;
         ties += k == kth;
     });
-    int tie = sel_scan(ties, sums2, lane, wave, &total);
-    const int stay0 = sel_scan(greater, sums, lane, wave, &total) + min(tie, left);   // rows before j0 that stay
+    const int2 before = sel_scan(ties, greater, sums[3], lane, wave);
+    int tie = before.x;
+    const int stay0 = before.y + min(tie, left);    // rows before j0 that stay
     // rows before the budget that stay: its thread knows
     {
         int st = stay0, t = tie;
@@ -1530,28 +1539,33 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
     __syncthreads();
     const int first = s_first;
     const size_t list = (size_t)item * a.most;
+    int* const from = a.move_here ? lds_from : a.from + list;
+    int* const to = a.move_here ? lds_to : a.to + list;
     int st = stay0;
     each([&](int j, uint32_t k) {
         const bool stay = k > kth || (k == kth && tie++ < left);
         if (j < a.budget) {
-            if (!stay) a.to[list + j - st] = j;
+            if (!stay) to[j - st] = j;
         } else if (stay) {
-            a.from[list + st - first] = j;
+            from[st - first] = j;
         }
         st += stay;
     });
     const int moves = a.budget - first;
-    if (tid == 0) a.count[item] = moves;
-    if (!a.move_here) return;
-    // the lists and the copies above are there before a row is moved
+    if (!a.move_here) {
+        if (tid == 0) a.count[item] = moves;
+        return;
+    }
+    // the copies above are there before a row is moved
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    move_rows(a, r, h, moves, 0, kSelThreads / (a.hd / 8));
+    move_rows(a, r, h, lds_from, lds_to, moves, 0, kSelThreads / (a.hd / 8));
 }
 
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
     const int h = blockIdx.y, r = blockIdx.z, rows = 256 / (a.hd / 8);
-    move_rows(a, r, h, a.count[r * a.p.nkv + h], blockIdx.x * rows, gridDim.x * rows);
+    const size_t item = (size_t)r * a.p.nkv + h;
+    move_rows(a, r, h, a.from + item * a.most, a.to + item * a.most, a.count[item], blockIdx.x * rows, gridDim.x * rows);
 }
 
 // ---- shapes -----------------------------------------------------------------------------
