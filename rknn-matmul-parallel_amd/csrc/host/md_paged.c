@@ -24,7 +24,7 @@ static int check_cache(const MdxPagedCache* c, const char* fn) {
     REFUSE_IF(c->type != MDX_TYPE_F16 && c->type != MDX_TYPE_BF16, "unknown type");
     REFUSE_IF(c->num_kv_heads < 1 || c->num_q_heads < 1 || c->num_q_heads % c->num_kv_heads,
               "num_q_heads has to be a multiple of num_kv_heads");
-    REFUSE_IF(c->num_q_heads > 65535, "too many heads");
+    REFUSE_IF(c->num_q_heads > 16384, "too many heads");
     REFUSE_IF(c->n_pages < 1 || !c->k_pages || !c->v_pages, "no pages");
     REFUSE_IF(misaligned(c->k_pages, 16) || misaligned(c->v_pages, 16), "pages have to be 16-byte aligned");
     REFUSE_IF(misaligned(c->mass, 16) || misaligned(c->pos, 16), "mass and pos have to be 16-byte aligned");
@@ -60,7 +60,8 @@ static int check_rows(const MdxPagedCache* c, const void* p, long long stride, c
 
 /* a scale of 0 is 1 / sqrt(head_dim) */
 static int check_scale(float scale, const char* fn) {
-    REFUSE_IF(!(scale >= 0.0f) || isinf(scale), "scale has to be positive, or 0 for 1 / sqrt(head_dim)");
+    REFUSE_IF(scale != 0.0f && !(scale >= 1.2e-38f && scale <= 1e30f),
+              "scale has to be 1.2e-38 to 1e30, or 0 for 1 / sqrt(head_dim)");
     return 0;
 }
 static float scale_of(const MdxPagedCache* c, float scale) {
@@ -115,6 +116,7 @@ int mdx_paged_attention(const MdxPagedCache* c, const MdxPagedBatch* b, const vo
     if (!rc) rc = check_rows(c, out, out_stride, fn, "no out");
     if (!rc) rc = check_workspace(workspace, workspace_bytes, mdx_paged_attn_scratch(c, b), fn);
     if (rc) return rc;
+    REFUSE_IF(q == out, "out has to be apart from q");
     REFUSE_IF(misaligned(lse, 4), "lse has to be 4-byte aligned");
     return mdx_launch_paged_attn(c, b, q, q_stride, scale_of(c, scale), out, out_stride, lse, workspace, stream);
 }

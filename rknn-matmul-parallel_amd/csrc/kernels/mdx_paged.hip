@@ -135,7 +135,9 @@ __device__ __forceinline__ float4_t mfma16(__bf16, u32x4_t a, u32x4_t b, float4_
 // One workgroup per new row; HD/4 lanes per head, four values each, so that a
 // head is read with 16-byte loads, its sum of squares is a few cross-lane adds
 // and a rotation's partner is in this lane (pairs) or HD/8 lanes away (halves).
-// Reads and writes are all it does: 4 + 2 bytes per value.
+// Reads and writes are all it does: 4 + 2 bytes per value; four rounds of loads are
+// issued before the request is looked up (one round at a time, after it: 4096 rows of
+// 16 + 2 x 8 heads of 128 25.5 us, so XX).
 struct AppendArgs {
     Paged p;
     const float* qkv;
@@ -153,71 +155,87 @@ struct AppendArgs {
 
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
-    constexpr int LPH = HD / 4;            // lanes per head
+    constexpr int LPH = HD / 4, HPB = 256 / LPH;   // lanes per head, heads per round
+    constexpr int AHEAD = 4;                        // rounds whose loads are issued together
     const Paged& p = a.p;
     const int t = blockIdx.x, lane = threadIdx.x & 63;
+    const int l = threadIdx.x % LPH, heads = p.nq + 2 * p.nkv;
+    const float* row = a.qkv + (size_t)t * a.qkv_stride;
+    float4 v[AHEAD];
+    auto load = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            v[i] = *reinterpret_cast<const float4*>(row + (size_t)min(h0 + HPB * i + (int)threadIdx.x / LPH, heads - 1) * HD + 4 * l);
+    };
+    // the row itself depends on nothing that has to be looked up first
+    load(0);
+    const int pos = fixed(a.positions, t);
     const int r = find_req(p, t, lane);
     if (r >= p.n_req) return;
     const Req q = req_of(p, r);
     const int i = t - q.start;
-    const int pos = a.positions[t];
     if (i < 0 || i >= min(q.n, p.max_q) || pos < 0 || pos >= a.max_pos) return;
     const int j = q.base + i;              // cache row
-    const bool held = j >= 0 && j < p.limit;
-    const int l = threadIdx.x % LPH, heads = p.nq + 2 * p.nkv;
-    const float* row = a.qkv + (size_t)t * a.qkv_stride;
-    const float* cr = a.cos_t + (size_t)pos * (HD / 2);
-    const float* sr = a.sin_t + (size_t)pos * (HD / 2);
-    for (int h0 = 0; h0 < heads; h0 += 256 / LPH) {
-        const int h = h0 + threadIdx.x / LPH;
-        const bool hv = h < heads;
-        float4 x = *reinterpret_cast<const float4*>(row + (size_t)min(h, heads - 1) * HD + 4 * l);
-        const float* nw = h < p.nq ? a.q_norm : a.k_norm;
-        const bool turn = h < p.nq + p.nkv;
-        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
-        ss = group_sum(ss, LPH);
-        if (turn && nw) {
-            const float rms = 1.0f / sqrtf(ss / (float)HD + a.eps);
-            const float4 w = *reinterpret_cast<const float4*>(nw + 4 * l);
-            x.x = (x.x * rms) * w.x;
-            x.y = (x.y * rms) * w.y;
-            x.z = (x.z * rms) * w.z;
-            x.w = (x.w * rms) * w.w;
-        }
-        if (a.style == 0) {
-            if (turn) {
-                const float2 c = *reinterpret_cast<const float2*>(cr + 2 * l);
-                const float2 s = *reinterpret_cast<const float2*>(sr + 2 * l);
-                x = make_float4(x.x * c.x - x.y * s.x, x.y * c.x + x.x * s.x, x.z * c.y - x.w * s.y,
-                                x.w * c.y + x.z * s.y);
+    const long long slot = j >= 0 && j < p.limit ? pool_row(p, r, 0, j) : -1;
+    // this lane's part of the tables: for pairs its two, for halves the four it shares
+    const size_t at = (size_t)pos * (HD / 2) + (a.style == 0 ? 2 * l : 4 * (l % (LPH / 2)));
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f), s = c;
+    if (a.style == 0) {
+        const float2 c2 = *reinterpret_cast<const float2*>(a.cos_t + at), s2 = *reinterpret_cast<const float2*>(a.sin_t + at);
+        c.x = c2.x;
+        c.y = c2.y;
+        s.x = s2.x;
+        s.y = s2.y;
+    } else {
+        c = *reinterpret_cast<const float4*>(a.cos_t + at);
+        s = *reinterpret_cast<const float4*>(a.sin_t + at);
+        if (l < LPH / 2) s = make_float4(-s.x, -s.y, -s.z, -s.w);
+    }
+    for (int h0 = 0; h0 < heads; h0 += HPB * AHEAD) {
+        if (h0 > 0) load(h0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int h = h0 + HPB * i + threadIdx.x / LPH;
+            if (h0 + HPB * i >= heads) break;
+            float4 x = v[i];
+            const float* nw = h < p.nq ? a.q_norm : a.k_norm;
+            const bool turn = h < p.nq + p.nkv;
+            float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
+            ss = group_sum(ss, LPH);
+            if (turn && nw) {
+                const float rms = 1.0f / sqrtf(ss / (float)HD + a.eps);
+                const float4 w = *reinterpret_cast<const float4*>(nw + 4 * l);
+                x.x = (x.x * rms) * w.x;
+                x.y = (x.y * rms) * w.y;
+                x.z = (x.z * rms) * w.z;
+                x.w = (x.w * rms) * w.w;
             }
-        } else {
-            float4 y;
-            y.x = __shfl_xor(x.x, LPH / 2, kWave);
-            y.y = __shfl_xor(x.y, LPH / 2, kWave);
-            y.z = __shfl_xor(x.z, LPH / 2, kWave);
-            y.w = __shfl_xor(x.w, LPH / 2, kWave);
-            if (turn) {
-                const int lo = l % (LPH / 2);
-                const float4 c = *reinterpret_cast<const float4*>(cr + 4 * lo);
-                float4 s = *reinterpret_cast<const float4*>(sr + 4 * lo);
-                if (l < LPH / 2) s = make_float4(-s.x, -s.y, -s.z, -s.w);
-                x = make_float4(x.x * c.x + y.x * s.x, x.y * c.y + y.y * s.y, x.z * c.z + y.z * s.z,
-                                x.w * c.w + y.w * s.w);
+            if (a.style == 0) {
+                if (turn)
+                    x = make_float4(x.x * c.x - x.y * s.x, x.y * c.x + x.x * s.x, x.z * c.y - x.w * s.y,
+                                    x.w * c.y + x.z * s.y);
+            } else {
+                float4 y;
+                y.x = __shfl_xor(x.x, LPH / 2, kWave);
+                y.y = __shfl_xor(x.y, LPH / 2, kWave);
+                y.z = __shfl_xor(x.z, LPH / 2, kWave);
+                y.w = __shfl_xor(x.w, LPH / 2, kWave);
+                if (turn)
+                    x = make_float4(x.x * c.x + y.x * s.x, x.y * c.y + y.y * s.y, x.z * c.z + y.z * s.z,
+                                    x.w * c.w + y.w * s.w);
             }
-        }
-        if (!hv) continue;
-        const uint2 o = make_uint2(pack16<T>(x.x, x.y), pack16<T>(x.z, x.w));
-        if (h < p.nq) {
-            *reinterpret_cast<uint2*>(a.q_out + (size_t)t * a.q_stride + (size_t)h * HD + 4 * l) = o;
-        } else if (held) {
-            const bool is_k = h < p.nq + p.nkv;
-            const long long to = pool_row(p, r, is_k ? h - p.nq : h - p.nq - p.nkv, j);
-            if (to < 0) continue;
-            *reinterpret_cast<uint2*>((is_k ? p.kp : p.vp) + to * HD + 4 * l) = o;
-            if (is_k && l == 0) {
-                if (p.mass) p.mass[to] = 0.0f;
-                if (p.pos) p.pos[to] = pos;
+            if (h >= heads) continue;
+            const uint2 o = make_uint2(pack16<T>(x.x, x.y), pack16<T>(x.z, x.w));
+            if (h < p.nq) {
+                *reinterpret_cast<uint2*>(a.q_out + (size_t)t * a.q_stride + (size_t)h * HD + 4 * l) = o;
+            } else if (slot >= 0) {
+                const bool is_k = h < p.nq + p.nkv;
+                const long long to = slot + ((long long)(is_k ? h - p.nq : h - p.nq - p.nkv) << p.shift);
+                *reinterpret_cast<uint2*>((is_k ? p.kp : p.vp) + to * HD + 4 * l) = o;
+                if (is_k && l == 0) {
+                    if (p.mass) p.mass[to] = 0.0f;
+                    if (p.pos) p.pos[to] = pos;
+                }
             }
         }
     }
@@ -1580,7 +1598,8 @@ constexpr int kWideJoin = 16;
 struct Plan {
     int short_max;
     int tiles, waves, splits, split_keys, short_rows;    // k_paged_attn (tiles 0: not launched)
-    int blocks, chunk_splits, chunk_keys;                // k_paged_chunk (blocks 0: not launched)
+    long long blocks;
+    int chunk_splits, chunk_keys;                        // k_paged_chunk (blocks 0: not launched)
 };
 Plan attn_plan(const Paged& p) {
     Plan s = {};
@@ -1607,7 +1626,7 @@ Plan attn_plan(const Paged& p) {
         long long n = chunk_blocks;
         const long long each = (long long)p.n_req * cdiv(rows, kRows);
         if (n > each) n = each;
-        s.blocks = (int)n;
+        s.blocks = n;
         long long want = kCus / (n * p.nkv);
         const long long most = cdiv(limit, 512);
         want = want < 1 ? 1 : (want > most ? most : want);
@@ -1642,7 +1661,7 @@ void append_launch(const AppendArgs& a, hipStream_t s) {
 template <int HD, class T>
 void attn_launch(const AttnArgs& a, const Plan& s, hipStream_t st) {
     if (s.blocks)
-        hipLaunchKernelGGL((k_paged_chunk<HD, T>), dim3(s.blocks * a.p.nkv, s.chunk_splits), dim3(HD == 256 ? 256 : 512),
+        hipLaunchKernelGGL((k_paged_chunk<HD, T>), dim3((unsigned)(s.blocks * a.p.nkv), s.chunk_splits), dim3(HD == 256 ? 256 : 512),
                            0, st, a);
     const dim3 grid(s.splits, a.p.nkv * s.tiles, a.p.n_req);
     if (s.tiles && s.waves == 8) hipLaunchKernelGGL((k_paged_attn<HD, T, 8>), grid, dim3(512), 0, st, a);
@@ -1722,7 +1741,7 @@ int mdx_launch_paged_attn(const MdxPagedCache* c, const MdxPagedBatch* b, const 
     a.part_o = a.short_o + ns * hd;
     a.short_ml = (float2*)(a.part_o + nc * hd);
     a.part_ml = a.short_ml + ns;
-    if ((long long)s.blocks * a.p.nkv > 0x7fffffffLL) return mdxrt_refuse(-1, "mdx_paged_attention: too many rows");
+    if (s.blocks * a.p.nkv > 0x7fffffLL) return mdxrt_refuse(-1, "mdx_paged_attention: too many rows");
     MDX_PAGED_HD(attn_launch, a, s, (hipStream_t)stream);
     return mdxrt_launched("mdx_paged_attention");
 }

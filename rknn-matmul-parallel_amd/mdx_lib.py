@@ -392,7 +392,8 @@ PAGED_TYPES = {"fp16": 0, "bf16": 1}
 
 
 def _dev(a):
-    return a.data_ptr() if hasattr(a, "data_ptr") else a
+    ptr = getattr(a, "data_ptr", None)
+    return a if ptr is None else ptr()
 
 
 def paged_cache(dtype, num_q_heads, num_kv_heads, head_dim, page_size, n_pages, k_pages, v_pages, mass=None,
@@ -409,10 +410,13 @@ def paged_batch(n_req, n_tokens, max_q_len, max_kv_len, max_pages, q_start, kv_l
 def paged_append(cache, batch, qkv, positions, cos, sin, max_pos, q_out, q_norm=None, k_norm=None, eps=1e-6,
                  rope_style=0, qkv_stride=None, q_stride=None, stream=None) -> None:
     """mdx_paged_append; strides default to rows without gaps."""
-    qd, kvd = cache.num_q_heads * cache.head_dim, cache.num_kv_heads * cache.head_dim
-    _check(lib().mdx_paged_append(cache, batch, _dev(qkv), qd + 2 * kvd if qkv_stride is None else qkv_stride,
-                                  _dev(positions), _dev(q_norm), _dev(k_norm), eps, _dev(cos), _dev(sin), max_pos,
-                                  rope_style, _dev(q_out), qd if q_stride is None else q_stride, stream), "paged_append")
+    if qkv_stride is None:
+        qkv_stride = (cache.num_q_heads + 2 * cache.num_kv_heads) * cache.head_dim
+    if q_stride is None:
+        q_stride = cache.num_q_heads * cache.head_dim
+    _check(lib().mdx_paged_append(cache, batch, _dev(qkv), qkv_stride, _dev(positions), _dev(q_norm), _dev(k_norm), eps,
+                                  _dev(cos), _dev(sin), max_pos, rope_style, _dev(q_out), q_stride, stream),
+           "paged_append")
 
 
 def paged_attention_workspace(cache, batch) -> int:

@@ -24,7 +24,7 @@ def _batch(mdx, **over):
 
 CALLS = {
     "append": lambda m, c, b, **k: m.paged_append(c, b, **{**dict(qkv=A, positions=A, cos=A, sin=A, max_pos=64, q_out=A), **k}),
-    "attention": lambda m, c, b, **k: m.paged_attention(c, b, **{**dict(q=A, out=A, workspace=A, workspace_bytes=1 << 40), **k}),
+    "attention": lambda m, c, b, **k: m.paged_attention(c, b, **{**dict(q=A, out=2 * A, workspace=A, workspace_bytes=1 << 40), **k}),
     "mass": lambda m, c, b, **k: m.paged_mass(c, b, **{**dict(q=A, lse=A, workspace=A, workspace_bytes=1 << 40), **k}),
     "evict": lambda m, c, b, **k: m.paged_evict(c, b, **{**dict(budget=8, sink=2, recent=4, mass_out=A, pos_out=A, workspace=A, workspace_bytes=1 << 40), **k}),
 }
@@ -40,7 +40,7 @@ def _refused(mdx, call, c, b, rc, says, **k):
 @pytest.mark.parametrize("over,rc,says", [
     (dict(dtype=2), -1, "unknown type"), (dict(dtype=-1), -1, "unknown type"),
     (dict(num_q_heads=5), -1, "multiple of num_kv_heads"), (dict(num_kv_heads=0), -1, "multiple of num_kv_heads"),
-    (dict(num_q_heads=0), -1, "multiple of num_kv_heads"), (dict(num_q_heads=65536), -1, "too many heads"),
+    (dict(num_q_heads=0), -1, "multiple of num_kv_heads"), (dict(num_q_heads=16386), -1, "too many heads"),
     (dict(head_dim=96), -5, "head_dim"), (dict(head_dim=0), -5, "head_dim"),
     (dict(page_size=8), -5, "page_size"), (dict(page_size=24), -5, "page_size"), (dict(page_size=2048), -5, "page_size"),
     (dict(page_size=0), -5, "page_size"), (dict(page_size=-16), -5, "page_size"),
@@ -76,7 +76,8 @@ def test_refused_rows_of_a_batch(mdx, call, over, says):
     ("append", dict(q_stride=260), "stride"),
     ("attention", dict(q=None), "no q"), ("attention", dict(q=A + 2), "aligned"), ("attention", dict(out=None), "no out"),
     ("attention", dict(q_stride=255), "stride"), ("attention", dict(out_stride=257), "stride"), ("attention", dict(scale=-1.0), "scale"),
-    ("attention", dict(scale=float("nan")), "scale"), ("attention", dict(scale=float("inf")), "scale"), ("attention", dict(lse=A + 1), "lse"),
+    ("attention", dict(scale=float("nan")), "scale"), ("attention", dict(scale=1e-39), "scale"), ("attention", dict(scale=2e30), "scale"),
+    ("attention", dict(q=A, out=A), "apart"), ("attention", dict(scale=float("inf")), "scale"), ("attention", dict(lse=A + 1), "lse"),
     ("mass", dict(q=None), "no q"), ("mass", dict(lse=None), "lse"), ("mass", dict(q_stride=0), "stride"), ("mass", dict(scale=-0.5), "scale"),
     ("evict", dict(budget=-1), "budget"), ("evict", dict(sink=-1), "budget"), ("evict", dict(recent=-1), "budget"),
     ("evict", dict(sink=5), "budget"), ("evict", dict(recent=2 ** 31 - 1), "budget"), ("evict", dict(mass_out=None), "mass_out"),
@@ -106,7 +107,7 @@ def test_refused_workspaces(mdx):
 def test_null_structs_are_refused(mdx, call):
     L, p = mdx.lib(), C.c_void_p(A)
     fn = {"append": lambda c, b: L.mdx_paged_append(c, b, p, 512, p, None, None, 1e-6, p, p, 64, 0, p, 256, None),
-          "attention": lambda c, b: L.mdx_paged_attention(c, b, p, 256, 0.0, p, 256, None, p, 1 << 40, None),
+          "attention": lambda c, b: L.mdx_paged_attention(c, b, p, 256, 0.0, C.c_void_p(2 * A), 256, None, p, 1 << 40, None),
           "mass": lambda c, b: L.mdx_paged_mass(c, b, p, 256, 0.0, p, p, 1 << 40, None),
           "evict": lambda c, b: L.mdx_paged_evict(c, b, 8, 2, 4, p, p, p, 1 << 40, None)}[call]
     assert fn(None, _batch(mdx)) == -1 and fn(_cache(mdx), None) == -1
