@@ -231,4 +231,4 @@ def near(got_bits, ref, slack, dtype):
     if not np.array_equal(got[~fin & ~np.isnan(ref)], ref[~fin & ~np.isnan(ref)]):
         return np.inf
     bound = EPS[dtype] / 2 * (np.abs(ref) + slack) + slack + TINY[dtype] / 2
-    return float(np.max((np.abs(got - ref) - bound)[fin], initial=-1.0))
+    return float(np.max(np.abs(got[fin] - ref[fin]) - bound[fin], initial=-1.0))

@@ -25,7 +25,7 @@ def _check_attention(mdx, w, **k):
     assert near(out[taking_part], ref[taking_part], slack[taking_part], w.dtype) <= 0
     fin = np.isfinite(rlse[taking_part])
     assert np.array_equal(lse[taking_part][~fin], rlse[taking_part].astype(np.float32)[~fin], equal_nan=True)
-    assert np.all(np.abs(lse[taking_part] - rlse[taking_part])[fin] <= lslack[taking_part][fin])
+    assert np.all(np.abs(lse[taking_part][fin] - rlse[taking_part][fin]) <= lslack[taking_part][fin])
     return out, lse
 
 
@@ -167,6 +167,51 @@ def test_attention_large_and_small_values(mdx, gpu, dtype, std, q_std, new, kv):
     w = World(rng, dtype, 2, 2, 64, 16, new, kv, std=std, q_std=q_std).upload(mdx)
     _check_attention(mdx, w)
     _check_attention(mdx, w, scale=0.03)
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,hd", [("fp16", 16, 8, 64), ("bf16", 24, 8, 128)])
+def test_attention_chunks_beside_single_tokens(mdx, gpu, dtype, nq, nkv, hd):
+    """More blocks than CUs: chunks and short requests go through kernels of their own, both with splits."""
+    rng = np.random.default_rng(16)
+    new = [1] * 44
+    new[3], new[17], new[18], new[43] = 40, 17, 2, 33
+    kv = [int(x) for x in rng.integers(1, 120, 44) + np.array(new)]
+    kv[0], kv[3], kv[5] = 1100, 1300, 513
+    _check_attention(mdx, World(rng, dtype, nq, nkv, hd, 32, new, kv).upload(mdx))
+
+
+@pytest.mark.parametrize("requests", [64, 65, 150])
+def test_attention_many_requests(mdx, gpu, requests):
+    """More requests than a wave has lanes, empty ones among them."""
+    rng = np.random.default_rng(requests)
+    new = [int(x) for x in rng.choice([0, 1, 1, 1, 3, 40], requests)]
+    new[0], new[-1] = 70, 41
+    kv = [n + int(x) for n, x in zip(new, rng.integers(0, 60, requests))]
+    w = World(rng, "fp16", 2, 1, 64, 16, new, kv).upload(mdx)
+    _, lse = _check_attention(mdx, w)
+    _check_mass(mdx, w, np.nan_to_num(lse, nan=0.0, neginf=-np.inf))
+
+
+def test_attention_on_two_streams(mdx, gpu):
+    """Calls at once, each with its own workspace and outputs, against the same ones alone."""
+    H = _hip()
+    rng = np.random.default_rng(17)
+    worlds = [World(rng, "fp16", 8, 4, 128, 64, *x).upload(mdx) for x in (([1] * 8, [3000] * 8), ([300], [2000]), ([1, 60, 1], [700, 900, 20]))]
+    alone = [w.attention(mdx) for w in worlds]
+    streams = [C.c_void_p() for _ in worlds]
+    outs = []
+    for w, st in zip(worlds, streams):
+        assert H.hipStreamCreate(C.byref(st)) == 0
+        need = mdx.paged_attention_workspace(w.cache, w.batch)
+        outs.append((Dev(mdx, np.zeros(w.q.shape, np.uint16)), Dev(mdx, np.zeros((w.T, w.nq), np.float32)), Dev(mdx, np.zeros(max(need, 16), np.uint8)), need))
+    assert mdx.lib().mdx_device_synchronize() == 0
+    for _ in range(5):
+        for w, st, (o, l, ws, need) in zip(worlds, streams, outs):
+            mdx.paged_attention(w.cache, w.batch, w.d["q"], o, ws, need, lse=l, stream=st)
+    for (o, l, _, _), (a, b) in zip(outs, alone):
+        assert np.array_equal(o.get(), a) and np.array_equal(l.get(), b)
+    for st in streams:
+        assert H.hipStreamDestroy(st) == 0
 
 
 def test_attention_without_lse_gives_the_same(mdx, gpu):
@@ -445,9 +490,106 @@ def test_steps_together(mdx, gpu):
     assert held == [budget, budget] and seen == [54, 76]
 
 
+def test_pool_beyond_32_bits(mdx, gpu):
+    """Pages whose values lie more than 2^31 values and 2^32 bytes into the pool, through all four calls."""
+    rng = np.random.default_rng(23)
+    nq, nkv, hd, page, budget = 8, 8, 128, 1024, 40
+    w = World(rng, "bf16", nq, nkv, hd, page, [1, 70], [600, 90], extra_pages=0)
+    w.mass = rng.random(w.mass.shape).astype(np.float32)
+    w.upload(mdx)
+    off = 2100                                             # 2100 pages of 2 MiB
+    n = off + w.n_pages
+    L = mdx.lib()
+    big = {}
+    try:
+        for name in ("k", "v", "mass", "pos"):
+            big[name] = C.c_void_p()
+            per = w.d[name].a.nbytes // w.n_pages
+            assert L.mdx_device_malloc(C.byref(big[name]), n * per) == 0
+            assert L.mdx_memcpy_h2d(big[name].value + off * per, w.d[name].a.ctypes.data, w.d[name].a.nbytes) == 0
+        cache = mdx.paged_cache("bf16", nq, nkv, hd, page, n, *(big[x].value for x in ("k", "v", "mass", "pos")))
+        table = Dev(mdx, np.where(w.table >= 0, w.table + off, -1).astype(np.int32))
+        batch = mdx.paged_batch(w.R, w.T, w.max_q, w.max_kv, w.max_pages, w.d["q_start"], w.d["kv_len"], table)
+
+        def pages(name):
+            a = np.empty_like(w.d[name].a)
+            assert L.mdx_device_synchronize() == 0
+            assert L.mdx_memcpy_d2h(a.ctypes.data, big[name].value + off * (a.nbytes // w.n_pages), a.nbytes) == 0
+            return a
+
+        out, lse = Dev(mdx, np.zeros(w.q.shape, np.uint16)), Dev(mdx, np.zeros((w.T, nq), np.float32))
+        need = max(mdx.paged_attention_workspace(cache, batch), mdx.paged_mass_workspace(cache, batch), mdx.paged_evict_workspace(cache, batch, budget))
+        ws = Dev(mdx, np.zeros(max(need, 16), np.uint8))
+        qkv = rng.standard_normal((w.T, (nq + 2 * nkv) * hd)).astype(np.float32)
+        positions = np.concatenate([[599], np.arange(20, 90)]).astype(np.int32)
+        cos, sin = np.ones((600, hd // 2), np.float32), np.zeros((600, hd // 2), np.float32)
+        dev = [Dev(mdx, x) for x in (qkv, positions, cos, sin)]
+        mdx.paged_append(cache, batch, *dev, 600, w.d["q"])
+        w.q, w.k, w.v, w.mass, w.pos = w.d["q"].get(), pages("k"), pages("v"), pages("mass"), pages("pos")
+        _, _, k, dk, v = ref_append(w, qkv, positions, None, None, 0.0, cos, sin, 0)
+        for r in range(2):
+            for t, _, row in w.rows(r):
+                pg, slot = w.table[r, row // page], row % page
+                assert near(w.k[pg, :, slot], k[t], dk[t], "bf16") <= 0 and np.array_equal(w.v[pg, :, slot], to16(v[t].astype(np.float32), "bf16"))
+        mdx.paged_attention(cache, batch, w.d["q"], out, ws, ws.a.nbytes, lse=lse)
+        ref, _, slack, _ = w.ref_attention()
+        assert near(out.get(), ref, slack, "bf16") <= 0
+        mdx.paged_mass(cache, batch, w.d["q"], lse, ws, ws.a.nbytes)
+        mass, slack = w.ref_mass(lse.get().astype(np.float64))
+        w.mass = pages("mass")
+        assert np.all(np.abs(w.mass - mass) <= slack)
+        mdx.paged_evict(cache, batch, budget, 2, 10, big["mass"].value, big["pos"].value, ws, ws.a.nbytes)
+        want = w.ref_evict(budget, 2, 10, w.mass, w.pos)
+        assert all(np.array_equal(pages(x), y) for x, y in zip(("k", "v", "mass", "pos"), want))
+    finally:
+        for x in big.values():
+            L.mdx_device_free(x)
+
+
 def _hip():
     from test_zz_no_alloc import _hip as f
     return f()
+
+
+def test_captured_chunks(mdx, gpu):
+    """A chunk's attention and mass from one captured graph, replayed with other lengths of chunk and cache."""
+    L, H = mdx.lib(), _hip()
+    rng = np.random.default_rng(24)
+    w = World(rng, "fp16", 4, 2, 128, 32, [200, 40], [900, 700]).upload(mdx)
+    out, lse = Dev(mdx, np.zeros(w.q.shape, np.uint16)), Dev(mdx, np.zeros((w.T, 4), np.float32))
+    sizes = mdx.paged_attention_workspace(w.cache, w.batch), mdx.paged_mass_workspace(w.cache, w.batch)
+    ws = [Dev(mdx, np.full(max(n, 16), 0xff, np.uint8)) for n in sizes]
+    stream, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    assert H.hipStreamCreate(C.byref(stream)) == 0
+    try:
+        w.attention(mdx)                                   # a first call outside the capture
+        assert H.hipStreamBeginCapture(stream, 2) == 0
+        mdx.paged_attention(w.cache, w.batch, w.d["q"], out, ws[0], sizes[0], lse=lse, stream=stream)
+        mdx.paged_mass(w.cache, w.batch, w.d["q"], lse, ws[1], sizes[1], stream=stream)
+        assert H.hipStreamEndCapture(stream, C.byref(graph)) == 0
+        assert H.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+        for new, kv in (([200, 40], [900, 700]), ([1, 200], [900, 333]), ([17, 3], [17, 700]), ([0, 130], [5, 130])):
+            w.new, w.kv = new, kv
+            w.q_start, w.kv_len = np.array([0, new[0], sum(new)], np.int32), np.array(kv, np.int32)
+            w.d["q_start"].put(w.q_start)
+            w.d["kv_len"].put(w.kv_len)
+            w.d["mass"].put(w.mass)
+            assert L.mdx_device_synchronize() == 0
+            assert H.hipGraphLaunch(exe, stream) == 0
+            assert H.hipStreamSynchronize(stream) == 0
+            ref, rlse, slack, lslack = w.ref_attention()
+            n = sum(new)
+            got = lse.get()
+            assert near(out.get()[:n], ref[:n], slack[:n], "fp16") <= 0 and np.all(np.abs(got - rlse)[:n] <= lslack[:n])
+            mass, ms = w.ref_mass(got.astype(np.float64))
+            assert np.all(np.abs(w.d["mass"].get() - mass) <= ms)
+            w.attention(mdx)                               # other work between the replays
+    finally:
+        if exe.value:
+            H.hipGraphExecDestroy(exe)
+        if graph.value:
+            H.hipGraphDestroy(graph)
+        H.hipStreamDestroy(stream)
 
 
 def test_captured_steps(mdx, gpu):
