@@ -288,7 +288,8 @@ typedef struct {
     void* v_pages;
     float* mass;            /* [n_pages][num_kv_heads][page_size], 16-byte aligned: weight received
                                (NULL: not kept) */
-    int* pos;               /* the same: the row's position in its request (NULL: not kept) */
+    int* pos;               /* the same: the row's position in its request, not negative (NULL: not
+                               kept) */
 } MdxPagedCache;
 
 /* The new rows of n_req requests, request after request.  Row i of the
@@ -316,8 +317,8 @@ typedef struct {
  * (2i, 2i+1) for rope_style 0, (i, i + head_dim/2) for 1), all in fp32 and
  * rounded once.  K and V go to the row's place in its request's pages, with
  * mass 0 and pos positions[t] where those are kept; q to q_out ([n_tokens] rows,
- * q_stride values apart).  A row whose position is outside the tables is left
- * out. */
+ * q_stride values apart; apart from qkv).  A row whose position is outside the
+ * tables is left out. */
 int mdx_paged_append(const MdxPagedCache* cache, const MdxPagedBatch* batch, const float* qkv,
                      long long qkv_stride, const int* positions, const float* q_norm,
                      const float* k_norm, float eps, const float* cos_t, const float* sin_t,
@@ -327,7 +328,8 @@ int mdx_paged_append(const MdxPagedCache* cache, const MdxPagedBatch* batch, con
  * that row t sees, those up to itself (scale 0: 1 / sqrt(head_dim)); lse[t][h]
  * (NULL: not wanted) the natural logarithm of the sum of the exponentials.  A
  * row that sees nothing gets zeros and lse -inf.  Rows are q_stride / out_stride
- * values apart, lse rows num_q_heads. */
+ * values apart, lse rows num_q_heads.  out is apart from q.  scale is 0 or within
+ * 1.2e-38 .. 1e30. */
 size_t mdx_paged_attention_workspace(const MdxPagedCache* cache, const MdxPagedBatch* batch);
 int mdx_paged_attention(const MdxPagedCache* cache, const MdxPagedBatch* batch, const void* q,
                         long long q_stride, float scale, void* out, long long out_stride, float* lse,

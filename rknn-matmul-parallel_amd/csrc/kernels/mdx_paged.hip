@@ -136,8 +136,9 @@ __device__ __forceinline__ float4_t mfma16(__bf16, u32x4_t a, u32x4_t b, float4_
 // head is read with 16-byte loads, its sum of squares is a few cross-lane adds
 // and a rotation's partner is in this lane (pairs) or HD/8 lanes away (halves).
 // Reads and writes are all it does: 4 + 2 bytes per value; four rounds of loads are
-// issued before the request is looked up (one round at a time, after it: 4096 rows of
-// 16 + 2 x 8 heads of 128 25.5 us, so XX).
+// issued before the request is looked up (4096 rows of 16 + 2 x 8 heads of 128: 24.0
+// us, 4.3 TB/s, where a large copy reaches 4.7; looked up first 25.5).  One row is the
+// latency of two loads and a launch: 7.9 us with the host's part.
 struct AppendArgs {
     Paged p;
     const float* qkv;
@@ -255,7 +256,10 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 //                      j has the dims (HD/16) m + j, so a lane's outputs of all
 //                      products are contiguous.
 // Probabilities enter as the sum of two 16-bit values (22 bits in fp16, 16 in
-// bf16): the keys' bytes bound this kernel, not its products.
+// bf16): the keys' bytes bound this kernel, not its products.  64 requests of 4096
+// rows, 8 heads of 128: 140 us, 5.0 TB/s; one of 131072: 101 us, 5.3 TB/s, with the
+// join.  (A wave that requests its next tile ahead gains nothing: 138.0 us for 137.4,
+// and 9.2 for 8.8 over 512 rows.)
 //
 // Rows and their order: masks are -inf scores; V rows that no row of the tile
 // sees are zeroed as they are loaded.  What is left of a non-finite V value at a
@@ -283,10 +287,10 @@ struct AttnArgs {
     int chunk_splits, chunk_keys;
 };
 
-// Probabilities are 2^(c (s - ref) + lift); the difference comes first, so that
-// it is exact near the maximum however large the scores are.  The reference only
-// moves when a row's maximum has outgrown it by 2^8; the lift takes fp16 values
-// away from the subnormal ones.
+// Probabilities are 2^(c (s - ref) + lift).  The difference comes first, so that it
+// is exact near the maximum however large the scores are (k_paged_chunk does that
+// where c ref is large).  The reference only moves when a row's maximum has outgrown
+// it by 2^8; the lift takes fp16 values away from the subnormal ones.
 template <class T> constexpr float kLift = 0.0f;
 template <> constexpr float kLift<_Float16> = 7.0f;
 
@@ -551,11 +555,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_attn(AttnArgs a) {
 // Probabilities go in rounded to the type once (the output's own rounding is as
 // large, and a second part would cost half as many products again); the sums are
 // of the unrounded ones.
+// What bounds it: 2048 rows over 8192, 16 heads of 128 over 8, 155 us, 770 TFLOP/s.
+// The products alone take 97 us at the clock that their power leaves (a large library
+// product: 1108 TFLOP/s), and a fragment that feeds 32 rows asks LDS for the 128 bytes
+// per clock that it has; 64 rows a wave would halve that, but hold one wave per SIMD,
+// with nobody to run its exponentials beside.
 //
-// V rows that no row of the block sees are zeroed on their way to LDS.  Values
-// that are not finite at places that some rows see and others do not leave 0 * inf
-// behind: rows whose sum of weights is a number and whose output is not are
-// computed again by row_again, key by key in fp32.
+// Masked places have probability 0, but K and V values there that are not finite
+// leave 0 * inf behind: rows whose sum of weights is a number and whose output is
+// not are computed again by row_again, key by key in fp32.
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
@@ -1177,8 +1185,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_paged_join(AttnArgs a
 //   many (a chunk): a workgroup owns 64 keys (32 at 256 dimensions), its four
 //     waves take every fourth tile of 32 rows, the next tile's rows on their way
 //     during the products of this one, and their sums are added in LDS in order.
-//     515 rows over 4000, 8 heads over 4 of 64, two requests: 36 -> XX us against
-//     the other form, which waits for each tile's rows.
+//     515 rows over 4000, 8 heads over 4 of 64, two requests: 12.5 us, where the
+//     other form, which waits for each tile's rows, takes 34.5.  Half of it are the
+//     exponentials, of which there are as many as scores.  (Of 1, 2, 4, 8 and 16
+//     waves: 15.5, 19.6, 12.5, 17.9 and 29.5 us.)
 struct MassArgs {
     Paged p;
     const uint16_t* q;
@@ -1412,8 +1422,8 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, cons
 // by lane; protected rows are counted per thread).  One scan over the threads then tells each how many rows before its
 // own stay, and with that which gaps and fillers its rows are.
 // What bounds it is latency: the chain of loads (length, page, mass) and five
-// scans with their barriers.  4 requests x 8 heads of 16384 rows XX us, 32 x 8 of
-// 2049 XX us.
+// scans with their barriers.  4 requests x 8 heads of 16384 rows 18 us (and 12 for
+// the moves), 32 x 8 of 2049, moves included, 9.2 us.
 template <int C>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
     __shared__ int4 hist[kSelBins];
@@ -1607,7 +1617,7 @@ Plan attn_plan(const Paged& p) {
     const long long rows = (long long)p.max_q * p.G;
     s.short_rows = rows < kShort ? (int)rows : kShort;
     // A batch with chunks whose blocks leave CUs free takes its short requests along
-    // in them: XX -> XX us for 24 requests, ten of them with chunks.
+    // in them: 67 -> 48 us for 24 requests, ten of them with chunks.
     const long long chunk_blocks = (long long)p.n_tokens * p.G / kRows + p.n_req;
     s.short_max = rows > kShort && chunk_blocks * p.nkv <= kCus ? 0 : kShort;
     // With as many rows as all requests can have, none is expected to be short (one
