@@ -555,11 +555,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_attn(AttnArgs a) {
 // Probabilities go in rounded to the type once (the output's own rounding is as
 // large, and a second part would cost half as many products again); the sums are
 // of the unrounded ones.
-// What bounds it: 2048 rows over 8192, 16 heads of 128 over 8, 155 us, 770 TFLOP/s.
-// The products alone take 97 us at the clock that their power leaves (a large library
-// product: 1108 TFLOP/s), and a fragment that feeds 32 rows asks LDS for the 128 bytes
-// per clock that it has; 64 rows a wave would halve that, but hold one wave per SIMD,
-// with nobody to run its exponentials beside.
+// What bounds it: 2048 rows over 8192, 16 heads of 128 over 8, 148 us, 810 TFLOP/s (a
+// large library product: 1108).  Softmax and barriers alone take 96 us of it, with
+// the products beside them 105; the rest is the tiles' way into LDS.  64 rows a wave
+// would halve what is read from there, but need 416 registers besides addresses,
+// with one wave per SIMD, and did not fit without spills.
 //
 // Masked places have probability 0, but K and V values there that are not finite
 // leave 0 * inf behind: rows whose sum of weights is a number and whose output is
@@ -646,10 +646,13 @@ __device__ __forceinline__ void row_again(const Paged& p, int r, int kvh, const 
     *sum = l;
 }
 
-template <int HD, class T>
+template <int HD>
+constexpr int kTileKeys = HD == 256 ? 32 : 64;
+
+template <int HD, class T, bool WHOLE>
 __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_paged_chunk(AttnArgs a) {
     constexpr int GR = HD == 256 ? 1 : 2;           // groups of four waves
-    constexpr int KB = HD == 256 ? 32 : 64;         // keys per tile
+    constexpr int KB = kTileKeys<HD>;               // keys per tile
     constexpr int CH = HD / 8;                      // 16-byte chunks per row
     constexpr int DS = HD / 16, DT = HD / 32, KT = KB / 32;
     constexpr int U = KB * CH / 256;                // 16-byte loads per thread and tile
@@ -724,12 +727,11 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     const int pmask = (1 << p.shift) - 1;
     const int srow = tid / CH, sch = tid % CH;
     constexpr int NG = KB / 16;                     // 16-key groups of a tile
-    const bool whole = (1 << p.shift) >= KB;        // a tile lies in one page
     typedef int i4_t __attribute__((ext_vector_type(4)));
     i4_t pgv, pgk, pgn;                             // page numbers of the next V and K tiles, and of one more
     auto pages = [&](int kb) __attribute__((always_inline)) {
         pgn = i4_t(fixed(table, min(kb, kend - 1) >> p.shift));
-        if (!whole) {
+        if (!WHOLE) {
             pgn.y = fixed(table, min(kb + 16, kend - 1) >> p.shift);
             if constexpr (NG == 4) {
                 pgn.z = fixed(table, min(kb + 32, kend - 1) >> p.shift);
@@ -752,22 +754,20 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     unsigned goes[V];
 #pragma unroll
     for (int i = 0; i < V; i++) goes[i] = 2 * ((srow + i * RPU) * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU)));
-    auto load = [&](const uint16_t* src, i4_t pg, uint16_t* dst, int kb) __attribute__((always_inline)) {
+    auto base = [&](const uint16_t* src, int page, int key) __attribute__((always_inline)) -> const char* {
+        return reinterpret_cast<const char*>(src + ((((size_t)(there(page) ? page : 0) * p.nkv + kvh) << p.shift) + (key & pmask)) * HD);
+    };
+    auto go = [&](const char* from, uint16_t* dst, int i) __attribute__((always_inline)) {
         typedef __attribute__((address_space(1))) const void gptr_t;
         typedef __attribute__((address_space(3))) void lptr_t;
-        auto base = [&](int page, int key) __attribute__((always_inline)) -> const char* {
-            return reinterpret_cast<const char*>(src + ((((size_t)(there(page) ? page : 0) * p.nkv + kvh) << p.shift) + (key & pmask)) * HD);
-        };
-        auto go = [&](const char* from, int i) __attribute__((always_inline)) {
-            __builtin_amdgcn_global_load_lds((gptr_t*)from, (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
-        };
+        __builtin_amdgcn_global_load_lds((gptr_t*)from, (lptr_t*)(dst + (grp * KB + i * RPU + wave * RPW) * HD), 16, 0, 0);
+    };
+    // round i of a whole tile at `at`
+    auto go_whole = [&](const char* at, uint16_t* dst, int i) __attribute__((always_inline)) {
+        go(at + i / V * (V * RPU * HD * 2) + goes[i % V], dst, i);
+    };
+    auto load = [&](const uint16_t* src, i4_t pg, uint16_t* dst, int kb) __attribute__((always_inline)) {
         if (kb >= k1) return;
-        if (whole && kb + KB <= kend) {
-            const char* at = base(pg.x, kb);
-#pragma unroll
-            for (int i = 0; i < U; i++) go(at + i / V * (V * RPU * HD * 2) + goes[i % V], i);
-            return;
-        }
 #pragma unroll
         for (int i = 0; i < U; i++) {
             // this round's 16 keys: 2 i + wave / 2, i or i / 2
@@ -775,7 +775,7 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
             const int page = CH == 8 && (wave >> 1) ? pg[(even + 1) & 3] : pg[even];
             const int key = min(kb + 16 * (even + (CH == 8 ? wave >> 1 : 0)), (kend - 1) & ~15);
             const unsigned row = min((srow + i * RPU) & 15, kend - 1 - key);
-            go(base(page, key) + 2 * (row * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU))), i);
+            go(base(src, page, key) + 2 * (row * HD + 8 * (sch ^ lds_swap<HD>(srow + i * RPU))), dst, i);
         }
     };
     // where this lane reads: K rows c32 (+ 32 kt), chunk 2 d + hi; V rows 4 hi + ..
@@ -812,8 +812,10 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
 #pragma unroll
         for (int e = 0; e < 2; e++) vf[kk & 1][d][e] = lds_read_tr(vs + vat[d][e] + 16 * kk * HD);
     };
-    // s = scores of the K tile (its first fragments are in kf)
-    auto scores = [&](const uint16_t* ks) __attribute__((always_inline)) {
+    // s = scores of the K tile (its first fragments are in kf); issue(i) requests what
+    // goes beside product i of a phase
+    constexpr int NM = KB / 16 * DT;                // products with V of a tile, and as many with K
+    auto scores = [&](const uint16_t* ks, auto issue) __attribute__((always_inline)) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
@@ -824,6 +826,7 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
                 if (kt + 1 < KT) kload(ks, kt + 1, d);
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                 if (kt + 1 < KT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                issue(NM + kt * DS + d);
             }
         }
     };
@@ -894,7 +897,7 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         l = l + ((l4[0] + l4[1]) + (l4[2] + l4[3]));
     };
     // o += V tile . pf (its first fragments are in vf[0]); then the first of ks
-    auto values = [&](const uint16_t* vs, const uint16_t* ks) __attribute__((always_inline)) {
+    auto values = [&](const uint16_t* vs, const uint16_t* ks, auto issue) __attribute__((always_inline)) {
         constexpr int KK = KB / 16, KPD = (DS + DT - 1) / DT;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
@@ -911,13 +914,20 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
                     for (int x = KPD * d; x < KPD * (d + 1) && x < DS; x++) kload(ks, 0, x);
                     __builtin_amdgcn_sched_group_barrier(0x100, KPD, 0);
                 }
+                issue(kk * DT + d);
             }
     };
 
     // A group's phases: the softmax of tile t; then the products V of t and K of
     // t + 1.  The other group is one phase off, so that the SIMDs' matrix and
     // vector units are asked for by one of the two at a time.  Rows of t + 1 (V)
-    // and t + 2 (K) are requested at the beginning of the first phase.
+    // and t + 2 (K) are requested a few products apart in the second phase and are
+    // waited for before the next one.  (All at once at the beginning of the first phase
+    // they hold up the wave that asks: 2048 rows over 8192, 16 heads of 128 over 8, 156
+    // us for 148; 8 of 256 over 4, 257 for 225; 1024 rows, 32 of 64 over 8, 112 for 99.)
+    // Where a tile is of several pages or
+    // is not whole, they are requested at the beginning of the first phase and waited
+    // for at the end of the second.
     const int nt = (k1 - k0 + KB - 1) / KB, steps = (nt + GR - 1) / GR;
     int kb = k0 + grp * KB;                         // this group's tile
     if (threadIdx.x == 0) again = 0;
@@ -927,6 +937,12 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
+    auto barrier = [&]() __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto none = [](int) __attribute__((always_inline)) {};
     if (nt > 0) {
         pages(kb);
         turn_pages();
@@ -943,37 +959,59 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         if (grp < nt) {
 #pragma unroll
             for (int d = 0; d < DS; d++) kload(k_even, 0, d);
-            scores(k_even);
+            scores(k_even, none);
         }
         if (grp == 1) __syncthreads();
     }
+    bool pending = false;
+    auto first = [&](const uint16_t* vs) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) vload(vs, 0, d);
+    };
     for (int t0 = 0; t0 < steps; t0 += 2) {
 #pragma unroll
         for (int odd = 0; odd < 2; odd++) {
             const int t = (t0 + odd) * GR + grp;
             if (t0 + odd >= steps) break;
-            load(p.vp, pgv, odd ? v_even : v_odd, kb + GR * KB);
-            load(p.kp, pgk, odd ? k_odd : k_even, kb + 2 * GR * KB);
             bits2 = exist();
             pages(kb + 3 * GR * KB);
-            if (t < nt) {
-                softmax(kb, bits);
-#pragma unroll
-                for (int d = 0; d < DT; d++) vload(odd ? v_odd : v_even, 0, d);
+            uint16_t* const vn = odd ? v_even : v_odd;
+            uint16_t* const kn = odd ? k_odd : k_even;
+            const bool fast = WHOLE && kb + 2 * GR * KB + KB <= k1;
+            if (!fast) {
+                load(p.vp, pgv, vn, kb + GR * KB);
+                load(p.kp, pgk, kn, kb + 2 * GR * KB);
             }
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
+            if (t < nt) softmax(kb, bits);
+            if (pending) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                barrier();
+                first(odd ? v_odd : v_even);
+            } else {
+                first(odd ? v_odd : v_even);
+                barrier();
+            }
             // (after the last tile: the scores of one that nobody asks for)
             if (t < nt) {
-                values(odd ? v_odd : v_even, odd ? k_even : k_odd);
-                scores(odd ? k_even : k_odd);
+                const char* const va = base(p.vp, pgv.x, kb + GR * KB);
+                const char* const ka = base(p.kp, pgk.x, kb + 2 * GR * KB);
+                auto issue = [&](int i) __attribute__((always_inline)) {
+                    if (i % (NM / U) != 0) return;
+                    i /= NM / U;
+                    if (!fast) return;
+                    if (i < U) go_whole(va, vn, i);
+                    else go_whole(ka, kn, i - U);
+                };
+                values(odd ? v_odd : v_even, odd ? k_even : k_odd, issue);
+                scores(odd ? k_even : k_odd, issue);
             }
             turn_pages();
             bits = bits1;
             bits1 = bits2;
             kb += GR * KB;
-            arrived();
+            if (!fast) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            pending = fast;
+            barrier();
         }
     }
     if (GR == 2 && grp == 0 && nt > 0) __syncthreads();
@@ -1670,9 +1708,11 @@ void append_launch(const AppendArgs& a, hipStream_t s) {
 
 template <int HD, class T>
 void attn_launch(const AttnArgs& a, const Plan& s, hipStream_t st) {
-    if (s.blocks)
-        hipLaunchKernelGGL((k_paged_chunk<HD, T>), dim3((unsigned)(s.blocks * a.p.nkv), s.chunk_splits), dim3(HD == 256 ? 256 : 512),
-                           0, st, a);
+    if (s.blocks) {
+        const dim3 blocks((unsigned)(s.blocks * a.p.nkv), s.chunk_splits), threads(HD == 256 ? 256 : 512);
+        if (1 << a.p.shift >= kTileKeys<HD>) hipLaunchKernelGGL((k_paged_chunk<HD, T, true>), blocks, threads, 0, st, a);
+        else hipLaunchKernelGGL((k_paged_chunk<HD, T, false>), blocks, threads, 0, st, a);
+    }
     const dim3 grid(s.splits, a.p.nkv * s.tiles, a.p.n_req);
     if (s.tiles && s.waves == 8) hipLaunchKernelGGL((k_paged_attn<HD, T, 8>), grid, dim3(512), 0, st, a);
     else if (s.tiles) hipLaunchKernelGGL((k_paged_attn<HD, T, 4>), grid, dim3(256), 0, st, a);
