@@ -925,9 +925,8 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
     // waited for before the next one.  (All at once at the beginning of the first phase
     // they hold up the wave that asks: 2048 rows over 8192, 16 heads of 128 over 8, 156
     // us for 148; 8 of 256 over 4, 257 for 225; 1024 rows, 32 of 64 over 8, 112 for 99.)
-    // Where a tile is of several pages or
-    // is not whole, they are requested at the beginning of the first phase and waited
-    // for at the end of the second.
+    // Where a tile is of several pages or is not whole, they are requested at the
+    // beginning of the first phase and waited for at the end of the second.
     const int nt = (k1 - k0 + KB - 1) / KB, steps = (nt + GR - 1) / GR;
     int kb = k0 + grp * KB;                         // this group's tile
     if (threadIdx.x == 0) again = 0;
@@ -973,14 +972,22 @@ __global__ __launch_bounds__(HD == 256 ? 256 : 512, HD == 256 ? 1 : 2) void k_pa
         for (int odd = 0; odd < 2; odd++) {
             const int t = (t0 + odd) * GR + grp;
             if (t0 + odd >= steps) break;
-            bits2 = exist();
-            pages(kb + 3 * GR * KB);
             uint16_t* const vn = odd ? v_even : v_odd;
             uint16_t* const kn = odd ? k_odd : k_even;
             const bool fast = WHOLE && kb + 2 * GR * KB + KB <= k1;
+            // (the wait for a page number goes where it delays less: 148 for 158 us, and
+            // with pages of 16 rows 44.4 for 48.9)
+            if (WHOLE) {
+                bits2 = exist();
+                pages(kb + 3 * GR * KB);
+            }
             if (!fast) {
                 load(p.vp, pgv, vn, kb + GR * KB);
                 load(p.kp, pgk, kn, kb + 2 * GR * KB);
+            }
+            if (!WHOLE) {
+                bits2 = exist();
+                pages(kb + 3 * GR * KB);
             }
             if (t < nt) softmax(kb, bits);
             if (pending) {
@@ -1655,7 +1662,7 @@ Plan attn_plan(const Paged& p) {
     const long long rows = (long long)p.max_q * p.G;
     s.short_rows = rows < kShort ? (int)rows : kShort;
     // A batch with chunks whose blocks leave CUs free takes its short requests along
-    // in them: 67 -> 48 us for 24 requests, ten of them with chunks.
+    // in them: 67 -> 48 us (now 44) for 24 requests, ten of them with chunks.
     const long long chunk_blocks = (long long)p.n_tokens * p.G / kRows + p.n_req;
     s.short_max = rows > kShort && chunk_blocks * p.nkv <= kCus ? 0 : kShort;
     // With as many rows as all requests can have, none is expected to be short (one

@@ -114,6 +114,28 @@ def test_attention_shared_and_missing_pages(mdx, gpu):
     assert not out[-1].any() and np.all(lse[-1] == -np.inf)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_attention_missing_pages_beside_a_page_of_nan(mdx, gpu, page, hd):
+    """Nothing of page 0 shows, which no request holds, where a chunk's pages do not exist (at the beginning, between others, at the end)."""
+    rng = np.random.default_rng(17)
+    w = World(rng, "fp16", 2, 1, hd, page, [70, 1, 130], [900, 700, 777])
+    free = (set(range(w.n_pages)) - set(w.table[w.table >= 0])).pop()
+    w.table[w.table == 0] = free
+    w.k[0], w.v[0] = (to16(np.full(w.k[0].shape, np.nan, np.float32), "fp16") for _ in range(2))
+    n = w.n_pages
+    w.table[0, 0], w.table[0, 256 // page], w.table[1, 1], w.table[2, 512 // page], w.table[2, -(-777 // page) - 1] = -1, n, -7, n + 5, -1
+    _check_attention(mdx, w.upload(mdx))
+
+
+@pytest.mark.parametrize("dtype,hd", [("bf16", 64), ("fp16", 128), ("bf16", 256)])
+@pytest.mark.parametrize("kv", [511, 512, 513, 640, 705, 1025])
+def test_attention_ends_of_long_chunks(mdx, gpu, dtype, hd, kv):
+    """Caches that end at, before and behind a tile, with several tiles on their way."""
+    rng = np.random.default_rng(kv)
+    _check_attention(mdx, World(rng, dtype, 4, 2, hd, 128, [33, kv - 300, 1], [kv, kv, 3]).upload(mdx))
+
+
 BAD = {"nan": np.nan, "inf": np.inf, "-inf": -np.inf}
 
 
