@@ -303,7 +303,8 @@ typedef struct {
     int n_req;
     int n_tokens;           /* new rows of all requests; rows behind q_start[n_req] are left alone */
     int max_q_len;          /* no request has more new rows (further ones are left out) */
-    int max_kv_len;         /* nor more cache rows, the new ones included (further ones are absent) */
+    int max_kv_len;         /* nor more cache rows, the new ones included (further ones are absent); this
+                               or max_pages * page_size is at most 2^29 */
     int max_pages;          /* entries per request in block_table */
     const int* q_start;     /* [n_req + 1], ascending from 0 */
     const int* kv_len;      /* [n_req] */

@@ -35,12 +35,15 @@ static int check_cache(const MdxPagedCache* c, const char* fn) {
     return 0;
 }
 
-/* `rows`: the call reads the new rows (q_start, n_tokens, max_q_len) */
-static int check_batch(const MdxPagedBatch* b, int rows, const char* fn) {
+/* `rows`: the call reads the new rows (q_start, n_tokens, max_q_len).  Kernels count a
+ * request's cache rows, rounded up to whole tiles, in 32 bits. */
+static int check_batch(const MdxPagedCache* c, const MdxPagedBatch* b, int rows, const char* fn) {
     REFUSE_IF(!b, "no batch");
     REFUSE_IF(b->n_req < 0 || b->n_req > 65535, "n_req has to be 0 to 65535");
     if (b->n_req == 0) return 0;
     REFUSE_IF(b->max_kv_len < 0 || b->max_pages < 0, "negative max_kv_len or max_pages");
+    REFUSE_IF(b->max_kv_len > 1 << 29 && (long long)b->max_pages * c->page_size > 1 << 29,
+              "a request has 2^29 cache rows at most");
     REFUSE_IF(!b->kv_len || !b->block_table, "no kv_len or block_table");
     REFUSE_IF(misaligned(b->kv_len, 4) || misaligned(b->block_table, 4) || misaligned(b->q_start, 4),
               "lengths and tables have to be 4-byte aligned");
@@ -80,7 +83,7 @@ int mdx_paged_append(const MdxPagedCache* c, const MdxPagedBatch* b, const float
                      long long q_stride, void* stream) {
     static const char fn[] = "mdx_paged_append";
     int rc = check_cache(c, fn);
-    if (!rc) rc = check_batch(b, 1, fn);
+    if (!rc) rc = check_batch(c, b, 1, fn);
     if (rc || b->n_req == 0 || b->n_tokens == 0) return rc;
     REFUSE_IF(!qkv || misaligned(qkv, 16), "qkv has to be there and 16-byte aligned");
     REFUSE_IF(qkv_stride < ((long long)c->num_q_heads + 2LL * c->num_kv_heads) * c->head_dim || qkv_stride % 4,
@@ -100,7 +103,7 @@ int mdx_paged_append(const MdxPagedCache* c, const MdxPagedBatch* b, const float
 
 size_t mdx_paged_attention_workspace(const MdxPagedCache* c, const MdxPagedBatch* b) {
     static const char fn[] = "mdx_paged_attention_workspace";
-    if (check_cache(c, fn) || check_batch(b, 1, fn) || b->n_req == 0 || b->n_tokens == 0) return 0;
+    if (check_cache(c, fn) || check_batch(c, b, 1, fn) || b->n_req == 0 || b->n_tokens == 0) return 0;
     return mdx_paged_attn_scratch(c, b);
 }
 
@@ -109,7 +112,7 @@ int mdx_paged_attention(const MdxPagedCache* c, const MdxPagedBatch* b, const vo
                         size_t workspace_bytes, void* stream) {
     static const char fn[] = "mdx_paged_attention";
     int rc = check_cache(c, fn);
-    if (!rc) rc = check_batch(b, 1, fn);
+    if (!rc) rc = check_batch(c, b, 1, fn);
     if (!rc) rc = check_scale(scale, fn);
     if (rc || b->n_req == 0 || b->n_tokens == 0) return rc;
     rc = check_rows(c, q, q_stride, fn, "no q");
@@ -123,7 +126,7 @@ int mdx_paged_attention(const MdxPagedCache* c, const MdxPagedBatch* b, const vo
 
 size_t mdx_paged_mass_workspace(const MdxPagedCache* c, const MdxPagedBatch* b) {
     static const char fn[] = "mdx_paged_mass_workspace";
-    if (check_cache(c, fn) || check_batch(b, 1, fn) || b->n_req == 0 || b->n_tokens == 0) return 0;
+    if (check_cache(c, fn) || check_batch(c, b, 1, fn) || b->n_req == 0 || b->n_tokens == 0) return 0;
     return mdx_paged_mass_scratch(c, b);
 }
 
@@ -131,7 +134,7 @@ int mdx_paged_mass(const MdxPagedCache* c, const MdxPagedBatch* b, const void* q
                    const float* lse, void* workspace, size_t workspace_bytes, void* stream) {
     static const char fn[] = "mdx_paged_mass";
     int rc = check_cache(c, fn);
-    if (!rc) rc = check_batch(b, 1, fn);
+    if (!rc) rc = check_batch(c, b, 1, fn);
     if (!rc) rc = check_scale(scale, fn);
     if (rc) return rc;
     REFUSE_IF(!c->mass, "the cache keeps no mass");
@@ -145,7 +148,7 @@ int mdx_paged_mass(const MdxPagedCache* c, const MdxPagedBatch* b, const void* q
 
 size_t mdx_paged_evict_workspace(const MdxPagedCache* c, const MdxPagedBatch* b, int budget) {
     static const char fn[] = "mdx_paged_evict_workspace";
-    if (check_cache(c, fn) || check_batch(b, 0, fn) || b->n_req == 0 || budget < 0) return 0;
+    if (check_cache(c, fn) || check_batch(c, b, 0, fn) || b->n_req == 0 || budget < 0) return 0;
     return mdx_paged_evict_scratch(c, b, budget);
 }
 
@@ -153,7 +156,7 @@ int mdx_paged_evict(const MdxPagedCache* c, const MdxPagedBatch* b, int budget, 
                     float* mass_out, int* pos_out, void* workspace, size_t workspace_bytes, void* stream) {
     static const char fn[] = "mdx_paged_evict";
     int rc = check_cache(c, fn);
-    if (!rc) rc = check_batch(b, 0, fn);
+    if (!rc) rc = check_batch(c, b, 0, fn);
     if (rc) return rc;
     REFUSE_IF(!c->mass || !c->pos, "the cache keeps no mass or no pos");
     REFUSE_IF(budget < 0 || sink < 0 || recent < 0 || (long long)sink + recent > budget,

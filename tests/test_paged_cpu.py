@@ -88,6 +88,16 @@ def test_refused_arguments(mdx, call, over, says):
     _refused(mdx, call, _cache(mdx), _batch(mdx), -1, says, **over)
 
 
+@pytest.mark.parametrize("call", list(CALLS))
+def test_refused_caches_beyond_32_bit_rows(mdx, call):
+    """More rows than kernels count; either bound on its own may be larger."""
+    big = _batch(mdx, max_kv_len=2 ** 31 - 1, max_pages=2 ** 29 // 16 + 1)
+    _refused(mdx, call, _cache(mdx), big, -1, "2^29")
+    assert mdx.paged_attention_workspace(_cache(mdx), big) == 0
+    for k in (dict(max_kv_len=2 ** 31 - 1, max_pages=2 ** 29 // 16), dict(max_kv_len=2 ** 29, max_pages=2 ** 31 - 1)):
+        assert 0 < mdx.paged_attention_workspace(_cache(mdx), _batch(mdx, **k)) < 1 << 40
+
+
 def test_refused_without_mass_or_pos(mdx):
     _refused(mdx, "mass", _cache(mdx, mass=None), _batch(mdx), -1, "keeps no mass")
     _refused(mdx, "evict", _cache(mdx, mass=None), _batch(mdx), -1, "no mass or no pos")
